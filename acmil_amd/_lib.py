@@ -17,6 +17,7 @@ ERRORS = {-1: "ACMIL_ERR_SHAPE", -2: "ACMIL_ERR_UNSUPPORTED", -3: "ACMIL_ERR_NUL
 MODE_F32, MODE_F16X3, MODE_F16 = 0, 1, 2
 MODES = {"fp32": MODE_F32, "f16x3": MODE_F16X3, "f16": MODE_F16}
 DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
+ACTS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4, "sigmoid": 5}
 MAX_TOKENS, MAX_TOKENS_FUSED, MAX_CLASSES = 16, 5, 16
 
 _vp, _i, _sz = C.c_void_p, C.c_int, C.c_size_t
@@ -122,6 +123,14 @@ SIGNATURES = {
     "acmil_ga_adamw_pack": (_i, [_vp] * 7 + [C.POINTER(_vp), C.POINTER(_vp), _vp, _vp] + [_vp] * 7 + [C.POINTER(_vp), C.POINTER(_vp), _vp, _vp] +
                             [_i] * 6 + [_vp] + [_vp, C.c_longlong, _vp, _vp, C.c_float, C.c_double, C.c_double, C.c_float, C.c_float, C.c_longlong,
                                                 _vp, _vp, _vp, _vp]),
+    "acmil_linear_act_workspace_bytes": (_sz, [_vp]),
+    "acmil_linear_act": (_i, [_vp, _vp, _sz, _vp]),
+    "acmil_linear_act_bwd_workspace_bytes": (_sz, [_vp]),
+    "acmil_linear_act_bwd": (_i, [_vp, _vp, _sz, _vp]),
+    "acmil_gated_ffn_workspace_bytes": (_sz, [_vp]),
+    "acmil_gated_ffn": (_i, [_vp, _vp, _sz, _vp]),
+    "acmil_gated_ffn_bwd_workspace_bytes": (_sz, [_vp]),
+    "acmil_gated_ffn_bwd": (_i, [_vp, _vp, _sz, _vp]),
 }
 
 
@@ -131,6 +140,24 @@ class AdamwArgs(C.Structure):
     _fields_ = [("flat_params", _vp), ("n_flat", C.c_longlong), ("exp_avg", _vp), ("exp_avg_sq", _vp), ("lr", C.c_float),
                 ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_float), ("weight_decay", C.c_float), ("step", C.c_longlong),
                 ("skipped", _vp), ("flag_report", _vp)]
+
+
+_ll = C.c_longlong
+
+
+class LinearArgs(C.Structure):
+    """struct acmil_linear_args (include/acmil_hip.h)"""
+    _fields_ = [("dtype", _i), ("act", _i), ("M", _i), ("K", _i), ("N", _i), ("x", _vp), ("ldx", _ll), ("W", _vp), ("ldw", _ll),
+                ("bias", _vp), ("res", _vp), ("ldr", _ll), ("y", _vp), ("ldy", _ll), ("pre", _vp), ("dy", _vp), ("lddy", _ll),
+                ("dx", _vp), ("dW", _vp), ("db", _vp)]
+
+
+class FfnArgs(C.Structure):
+    """struct acmil_ffn_args (include/acmil_hip.h)"""
+    _fields_ = [("dtype", _i), ("act", _i), ("M", _i), ("D", _i), ("F", _i), ("x", _vp), ("ldx", _ll), ("Wg", _vp), ("ldwg", _ll),
+                ("Wu", _vp), ("ldwu", _ll), ("Wd", _vp), ("ldwd", _ll), ("bg", _vp), ("bu", _vp), ("bd", _vp), ("res", _vp), ("ldr", _ll),
+                ("y", _vp), ("ldy", _ll), ("g", _vp), ("u", _vp), ("h", _vp), ("dy", _vp), ("lddy", _ll), ("dx", _vp), ("dWgu", _vp),
+                ("dWd", _vp), ("dbgu", _vp), ("dbd", _vp)]
 
 
 _lib = None

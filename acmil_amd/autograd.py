@@ -3,7 +3,7 @@ attention blocks and IBMIL (ACMIL_GA / ABMIL have their own fused backward: csrc
 
 Each Function's forward and backward are C-ABI kernels (csrc/gemm_f32.hip, csrc/transmil_train.hip, csrc/attn_generic.hip);
 autograd only sequences them and handles views / concatenation.  No torch math kernel runs over an O(N) tensor except
-copies (cat / pad / slicing / `+`) and the dropout mask.  CUDA fp32 tensors only (no CPU fallback).
+copies (cat / pad / slicing / `+`) and the dropout mask.  CUDA fp32 tensors only unless said otherwise (no CPU fallback).
 
   linear(x, W, b, relu)          nn.Linear (+ReLU)                    -> acmil_gemm_*            (transMIL.py:51,62; nystrom_attention.py:55,59)
   matmul(a, b, trans_a, trans_b) batched aten::matmul                 -> acmil_gemm_*            (nystrom_attention.py:113-133)
@@ -14,6 +14,8 @@ copies (cat / pad / slicing / `+`) and the dropout mask.  CUDA fp32 tensors only
   landmark_mean(src, l)          reduce(..., 'sum') / l               -> acmil_landmark_mean/_bwd
   gated_scores(h, ...)           Attention_Gated / Attn_Net_Gated     -> linear x3 + acmil_gate_fwd/_bwd
   attn_pool(h, A)                softmax over N, then P @ h           -> softmax_rows + matmul
+  linear_act(x, W, b, act, r)    16-bit act(x W^T + b) + r            -> acmil_linear_act/_bwd   (fp16 / bf16 tensors)
+  gated_ffn(x, Wg, Wu, Wd, ...)  16-bit gated feed-forward block      -> acmil_gated_ffn/_bwd    (fp16 / bf16 tensors)
 """
 from __future__ import annotations
 
@@ -321,3 +323,60 @@ class _MaskFill(torch.autograd.Function):
 def mask_fill(S: torch.Tensor, midx: torch.Tensor) -> torch.Tensor:
     return _MaskFill.apply(S, midx)
 
+
+
+class _LinearAct(torch.autograd.Function):
+    """acmil_linear_act / _bwd.  Kept for the backward: x, the weight and (for an activation) the pre-activations in FP32 -- a 16-bit copy
+    would add a rounding of act'(z) to the one of dz that the gradients already carry."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, act):
+        keep = act != "none" and any(ctx.needs_input_grad[:3])
+        out = ops.linear_act(x, weight, bias=bias, act=act, residual=residual, keep_pre=keep)
+        y, pre = out if keep else (out, None)
+        ctx.save_for_backward(x, weight, pre)
+        ctx.act = act
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, pre = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dx, dw, db = ops.linear_act_bwd(dy, x, weight, pre, act=ctx.act, need=need[:3]) if any(need[:3]) else (None, None, None)
+        return dx, dw, db, dy if need[3] else None, None
+
+
+def linear_act(x, weight, bias=None, act="none", residual=None):
+    """Differentiable ops.linear_act: act(x @ weight^T + bias) + residual for fp16 / bf16 tensors (no double backward)."""
+    return _LinearAct.apply(x, weight, bias, residual, act)
+
+
+class _GatedFfn(torch.autograd.Function):
+    """acmil_gated_ffn / _bwd.  Kept for the backward: x, the weights, both pre-activations in fp32 (as _LinearAct) and the gated features."""
+
+    @staticmethod
+    def forward(ctx, x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual, act):
+        keep = any(ctx.needs_input_grad[:7])
+        out = ops.gated_ffn(x, w_gate, w_up, w_down, b_gate=b_gate, b_up=b_up, b_down=b_down, act=act, residual=residual, keep=keep)
+        y, saved = out if keep else (out, (None, None, None))
+        ctx.save_for_backward(x, w_gate, w_up, w_down, *saved)
+        ctx.act = act
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, w_gate, w_up, w_down, g, u, h = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        grads = (None,) * 7
+        if any(need[:7]):
+            grads = ops.gated_ffn_bwd(dy, x, w_gate, w_up, w_down, (g, u, h), act=ctx.act, need_x=need[0], need_gate_up=need[1] or need[2],
+                                      need_down=need[3], need_gate_up_bias=need[4] or need[5], need_down_bias=need[6])
+        return tuple(t if n else None for t, n in zip(grads, need[:7])) + (dy if need[7] else None, None)
+
+
+def gated_ffn(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None, act="silu", residual=None):
+    """Differentiable ops.gated_ffn: (act(x @ w_gate^T + b_gate) * (x @ w_up^T + b_up)) @ w_down^T + b_down + residual for fp16 / bf16
+    tensors (no double backward)."""
+    return _GatedFfn.apply(x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual, act)

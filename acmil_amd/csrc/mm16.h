@@ -1,0 +1,195 @@
+// mm16.h -- shared by the 16-bit matrix products (mm16_kernel.h, mm16_rows.hip) and their C entries (mm16.hip): argument
+// blocks, the activations with their derivatives, and the epilogues on eight consecutive output columns.
+#pragma once
+#include "ga_common.h"
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+enum { MM_KC = 0, MM_KS = 1 };   // operand element (row, k) lies at row * ld + k (K contiguous) / at k * ld + row (K strided)
+// MM_ACT: y = act(v + bias) + residual, optionally v + bias kept.  MM_GATE: h = act(g + bg) * (u + bu), optionally both kept.
+// MM_GATE_BWD: v = dh -> dg = dh u act'(g), du = dh act(g).  MM_PART: raw fp32 sums of one K range for mm_join.
+enum { MM_ACT = 0, MM_GATE = 1, MM_GATE_BWD = 2, MM_PART = 3 };
+
+struct MmEpi {
+    int act, vec;                      // vec: every row that is touched starts on 16 bytes
+    const void *bias, *bias2;          // [N] in the operands' type, or null (bias2: of the second factor)
+    const void* res; long long ldr;    // [M, N] or null
+    void* out; long long ldo;          // MM_GATE_BWD: dg
+    void* out2;                        // MM_GATE_BWD: du (row stride ldo)
+    int npad;                          // >= N: columns N .. npad - 1 of out / out2 are written as zeros
+    float *pre, *pre2; long long ldp;  // fp32 [M, ldp]: kept pre-activations (written by MM_ACT / MM_GATE, read by MM_GATE_BWD), or null
+    float* part;                       // MM_PART: [splits][factors][M][ldpart]
+    int ldpart;
+};
+
+struct MmArgs {
+    const char *q0, *q1;               // operand of the output's rows; q1: second K segment
+    const char *p0, *p1;               // operand of the output's columns; p1: second K segment, or the second factor (DUAL)
+    long long ldq, ldp;                // leading dimensions in BYTES
+    int M, N;                          // output rows, columns (DUAL: of one factor)
+    int Kq, Kp;                        // valid K of either operand in one segment; what lies beyond reads as zero
+    int segs, splits;
+    int ntm, ntn;
+    MmEpi e;
+};
+
+static inline int mm_steps(const MmArgs& a) { return a.segs * ((((a.Kq > a.Kp) ? a.Kq : a.Kp) + 63) / 64); }
+int mm_launch_fwd(const MmArgs& a, bool bf, int epi, bool dual, bool large, hipStream_t st);     // P, Q with K contiguous
+int mm_launch_dgrad(const MmArgs& a, bool bf, int epi, bool large, hipStream_t st);              // P with K strided
+int mm_launch_wgrad(const MmArgs& a, bool bf, int epi, bool large, hipStream_t st);              // both with K strided
+// few rows: y / h of M <= MM_ROWS_MAX rows straight from memory, any alignment of 2 bytes
+#define MM_ROWS_MAX 32
+int mm_launch_rows(const MmArgs& a, bool bf, bool dual, hipStream_t st);
+
+template <bool BF> struct MmEl;
+template <> struct MmEl<true> { typedef __bf16 T; typedef bf16x8 V; };
+template <> struct MmEl<false> { typedef _Float16 T; typedef f16x8 V; };
+
+// sigmoid with one exponential; exp overflows to inf for very negative z and the quotient is then exactly 0
+__device__ __forceinline__ float mm_sigmoid(float z) { return 1.0f / (1.0f + __expf(-z)); }
+
+__device__ __forceinline__ float mm_act(int act, float z) {
+    switch (act) {
+        case ACMIL_ACT_RELU: return z < 0.0f ? 0.0f : z;                 // NaN stays NaN
+        case ACMIL_ACT_SILU: return z * mm_sigmoid(z);
+        case ACMIL_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+        case ACMIL_ACT_GELU_TANH: return z * mm_sigmoid(1.5957691216057308f * (z + 0.044715f * z * z * z));   // 0.5 z (1 + tanh t) = z sigmoid(2 t)
+        case ACMIL_ACT_SIGMOID: return mm_sigmoid(z);
+        default: return z;
+    }
+}
+
+// act(z) and act'(z)
+__device__ __forceinline__ float mm_act_slope(int act, float z, float& slope) {
+    switch (act) {
+        case ACMIL_ACT_RELU: slope = z > 0.0f ? 1.0f : 0.0f; return z < 0.0f ? 0.0f : z;
+        case ACMIL_ACT_SILU: { const float s = mm_sigmoid(z); slope = s * (1.0f + z * (1.0f - s)); return z * s; }
+        case ACMIL_ACT_GELU: {
+            const float c = 0.5f * (1.0f + erff(z * 0.70710678118654752f));
+            slope = c + z * 0.39894228040143268f * __expf(-0.5f * z * z);
+            return z * c;
+        }
+        case ACMIL_ACT_GELU_TANH: {
+            const float s = mm_sigmoid(1.5957691216057308f * (z + 0.044715f * z * z * z));
+            slope = s + z * s * (1.0f - s) * 1.5957691216057308f * (1.0f + 0.134145f * z * z);
+            return z * s;
+        }
+        case ACMIL_ACT_SIGMOID: { const float s = mm_sigmoid(z); slope = s * (1.0f - s); return s; }
+        default: slope = 1.0f; return z;
+    }
+}
+
+// eight at a time: one uniform branch on the activation, not one per element
+#define MM_EACH_ACT(CASE) \
+    switch (act) { \
+        case ACMIL_ACT_RELU: CASE(ACMIL_ACT_RELU) break; \
+        case ACMIL_ACT_SILU: CASE(ACMIL_ACT_SILU) break; \
+        case ACMIL_ACT_GELU: CASE(ACMIL_ACT_GELU) break; \
+        case ACMIL_ACT_GELU_TANH: CASE(ACMIL_ACT_GELU_TANH) break; \
+        case ACMIL_ACT_SIGMOID: CASE(ACMIL_ACT_SIGMOID) break; \
+        default: CASE(ACMIL_ACT_NONE) break; \
+    }
+__device__ __forceinline__ void mm_act8(int act, float* z) {
+#define MM_CASE(A) { _Pragma("unroll") for (int j = 0; j < 8; ++j) z[j] = mm_act(A, z[j]); }
+    MM_EACH_ACT(MM_CASE)
+#undef MM_CASE
+}
+__device__ __forceinline__ void mm_act_slope8(int act, const float* z, float* a, float* slope) {
+#define MM_CASE(A) { _Pragma("unroll") for (int j = 0; j < 8; ++j) a[j] = mm_act_slope(A, z[j], slope[j]); }
+    MM_EACH_ACT(MM_CASE)
+#undef MM_CASE
+}
+
+template <bool BF> __device__ __forceinline__ float mm_ld(const void* p, long long i) { return (float)((const typename MmEl<BF>::T*)p)[i]; }
+template <bool BF> __device__ __forceinline__ void mm_ld8(const void* p, long long i, float* v) {
+    const typename MmEl<BF>::V x = *(const typename MmEl<BF>::V*)((const typename MmEl<BF>::T*)p + i);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = (float)x[j];
+}
+template <bool BF> __device__ __forceinline__ void mm_st8(void* p, long long i, const float* v) {
+    typename MmEl<BF>::V x;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = (typename MmEl<BF>::T)v[j];      // one rounding to the tensors' type, to nearest even
+    *(typename MmEl<BF>::V*)((typename MmEl<BF>::T*)p + i) = x;
+}
+__device__ __forceinline__ void mm_ldf8(const float* p, float* v) {
+    const f32x4 a = *(const f32x4*)p, b = *(const f32x4*)(p + 4);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { v[j] = a[j]; v[4 + j] = b[j]; }
+}
+__device__ __forceinline__ void mm_stf8(float* p, const float* v) {
+    f32x4 a, b;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { a[j] = v[j]; b[j] = v[4 + j]; }
+    *(f32x4*)p = a; *(f32x4*)(p + 4) = b;
+}
+// eight values of a [N] vector or of a row, from column n: 16-byte loads where the row allows it, else one by one; nothing is read at or beyond N
+template <bool BF> __device__ __forceinline__ void mm_row8(const void* p, long long base, int n, int N, bool vec, float* v) {
+    if (vec && n + 8 <= N) { mm_ld8<BF>(p, base + n, v); return; }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = n + j < N ? mm_ld<BF>(p, base + n + j) : 0.0f;
+}
+// ... and their store; columns N .. npad - 1 become zero
+template <bool BF> __device__ __forceinline__ void mm_put8(void* p, long long base, int n, int N, int npad, bool vec, float* v) {
+    if (vec && n + 8 <= N) { mm_st8<BF>(p, base + n, v); return; }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+        if (n + j < npad) ((typename MmEl<BF>::T*)p)[base + n + j] = (typename MmEl<BF>::T)(n + j < N ? v[j] : 0.0f);
+}
+
+// The epilogues: row m, columns n .. n + 7 (n a multiple of 8).  Kept pre-activations have ldp >= round8(N): all eight are written.
+template <bool BF> __device__ __forceinline__ void mm_epi_act(const MmEpi& e, int m, int n, int N, float* v) {
+    const bool vec = e.vec != 0;
+    if (n >= e.npad) return;
+    if (e.bias) {
+        float b[8];
+        mm_row8<BF>(e.bias, 0, n, N, vec, b);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] += b[j];
+    }
+    if (e.pre) mm_stf8(e.pre + m * e.ldp + n, v);
+    mm_act8(e.act, v);
+    if (e.res) {
+        float r[8];
+        mm_row8<BF>(e.res, m * e.ldr, n, N, vec, r);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] += r[j];
+    }
+    mm_put8<BF>(e.out, m * e.ldo, n, N, e.npad, vec, v);
+}
+
+template <bool BF> __device__ __forceinline__ void mm_epi_gate(const MmEpi& e, int m, int n, int N, float* g, float* u) {
+    if (n >= e.npad) return;
+    if (e.bias) {
+        float b[8];
+        mm_row8<BF>(e.bias, 0, n, N, e.vec != 0, b);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) g[j] += b[j];
+    }
+    if (e.bias2) {
+        float b[8];
+        mm_row8<BF>(e.bias2, 0, n, N, e.vec != 0, b);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) u[j] += b[j];
+    }
+    if (e.pre) { mm_stf8(e.pre + m * e.ldp + n, g); mm_stf8(e.pre2 + m * e.ldp + n, u); }
+    mm_act8(e.act, g);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) g[j] *= u[j];
+    mm_put8<BF>(e.out, m * e.ldo, n, N, e.npad, true, g);      // h: rows of the library's own buffer, always on 16 bytes
+}
+
+template <bool BF> __device__ __forceinline__ void mm_epi_gate_bwd(const MmEpi& e, int m, int n, int N, float* v) {
+    if (n >= e.npad) return;
+    float g[8], u[8], a[8], slope[8];
+    mm_ldf8(e.pre + m * e.ldp + n, g);
+    mm_ldf8(e.pre2 + m * e.ldp + n, u);
+    mm_act_slope8(e.act, g, a, slope);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        g[j] = v[j] * u[j] * slope[j];
+        u[j] = v[j] * a[j];
+    }
+    mm_put8<BF>(e.out, m * e.ldo, n, N, e.npad, true, g);
+    mm_put8<BF>(e.out2, m * e.ldo, n, N, e.npad, true, u);
+}

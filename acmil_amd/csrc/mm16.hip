@@ -1,0 +1,410 @@
+// mm16.hip -- C entries of the 16-bit linear layer with a fused epilogue and of the gated feed-forward block, forward and
+// backward: shape and alignment handling, choice of tile and K split, and the small kernels around the products (padding copy,
+// dz = dy act'(z), column sums, the join of a split product).
+#include "mm16.h"
+
+// ------------------------------------------------------------------------------------------------ small kernels
+// src [rows, cols] (any leading dimension, any alignment of 2 bytes) -> dst [rows, ldd], ldd = round8(cols), zero-filled: the one
+// shape whose rows the LDS-DMA can fetch in 16-byte chunks.  Only matrices that are not already so pass through here.
+__global__ __launch_bounds__(256) void mm_pad_kernel(const short* __restrict__ src, long long lds, int rows, int cols, short* __restrict__ dst, int ldd) {
+    const int cpr = ldd / 8;
+    const long long total = (long long)rows * cpr;
+    for (long long i = blockIdx.x * 256LL + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+        const int r = (int)(i / cpr), c = (int)(i - (long long)r * cpr) * 8;
+        const short* s = src + r * lds + c;
+        short v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = c + j < cols ? s[j] : (short)0;
+        *(uint4*)(dst + (long long)r * ldd + c) = *(const uint4*)v;
+    }
+}
+
+// dz = dy act'(z), z kept in fp32; columns N .. ldz - 1 become zero
+template <bool BF>
+__global__ __launch_bounds__(256) void mm_dz_kernel(const void* __restrict__ dy, long long lddy, int vec, const float* __restrict__ z, long long ldp, int act,
+                                                    int M, int N, void* __restrict__ dz, int ldz) {
+    const int cpr = ldz / 8;
+    const long long total = (long long)M * cpr;
+    for (long long i = blockIdx.x * 256LL + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+        const int m = (int)(i / cpr), n = (int)(i - (long long)m * cpr) * 8;
+        float d[8], p[8];
+        mm_row8<BF>(dy, m * lddy, n, N, vec != 0, d);
+        mm_ldf8(z + m * ldp + n, p);
+        float a[8], slope[8];
+        mm_act_slope8(act, p, a, slope);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) d[j] *= slope[j];
+        mm_put8<BF>(dz, (long long)m * ldz, n, N, ldz, true, d);
+    }
+}
+
+// Column sums in two passes of fixed order: a workgroup adds its rows of 256 columns (8 row lanes x 32 chunks), part [gy][ldc] holds
+// what the second pass adds up.
+template <bool BF>
+__global__ __launch_bounds__(256) void mm_colsum_kernel(const void* __restrict__ x, long long ld, int rows, int cols8, float* __restrict__ part) {
+    __shared__ float red[8][32][9];
+    const int cx = threadIdx.x & 31, ry = threadIdx.x >> 5, c = (blockIdx.x * 32 + cx) * 8;
+    const int per = (rows + gridDim.y - 1) / gridDim.y, r0 = blockIdx.y * per, r1 = r0 + per < rows ? r0 + per : rows;
+    float s[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (c < cols8)
+        for (int r = r0 + ry; r < r1; r += 8) {
+            float v[8];
+            mm_ld8<BF>(x, r * ld + c, v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) s[j] += v[j];
+        }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) red[ry][cx][j] = s[j];
+    __syncthreads();
+    float t = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) t += red[k][threadIdx.x >> 3][threadIdx.x & 7];
+    const int col = blockIdx.x * 256 + threadIdx.x;
+    if (col < cols8) part[(size_t)blockIdx.y * cols8 + col] = t;
+}
+template <bool BF> __global__ __launch_bounds__(256) void mm_colsum_join_kernel(const float* __restrict__ part, int n, int cols8, int cols, void* __restrict__ out) {
+    const int c = blockIdx.x * 256 + threadIdx.x;
+    if (c >= cols) return;
+    float t = 0.0f;
+    for (int k = 0; k < n; ++k) t += part[(size_t)k * cols8 + c];
+    ((typename MmEl<BF>::T*)out)[c] = (typename MmEl<BF>::T)t;
+}
+
+// the K ranges of a split product, added in their order, and its epilogue
+template <bool BF, int EPI>
+__global__ __launch_bounds__(256) void mm_join_kernel(MmArgs a) {
+    const int cpr = a.e.ldpart / 8;
+    const long long total = (long long)a.M * cpr;
+    const long long i = blockIdx.x * 256LL + threadIdx.x;
+    if (i >= total) return;
+    const int m = (int)(i / cpr), n = (int)(i - (long long)m * cpr) * 8;
+    constexpr int NF = EPI == MM_GATE ? 2 : 1;
+    float v[NF][8];
+#pragma unroll
+    for (int f = 0; f < NF; ++f)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[f][j] = 0.0f;
+    const size_t plane = (size_t)a.M * a.e.ldpart;
+    for (int s = 0; s < a.splits; ++s)
+#pragma unroll
+        for (int f = 0; f < NF; ++f) {
+            float w[8];
+            mm_ldf8(a.e.part + (size_t)(s * NF + f) * plane + (size_t)m * a.e.ldpart + n, w);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[f][j] += w[j];
+        }
+    if constexpr (EPI == MM_GATE) mm_epi_gate<BF>(a.e, m, n, a.N, v[0], v[1]);
+    else if constexpr (EPI == MM_GATE_BWD) mm_epi_gate_bwd<BF>(a.e, m, n, a.N, v[0]);
+    else mm_epi_act<BF>(a.e, m, n, a.N, v[0]);
+}
+
+// ------------------------------------------------------------------------------------------------ host
+namespace {
+
+inline int r8(int n) { return (n + 7) & ~7; }
+
+// Hands out the caller's workspace; with a null base it only adds up what the same calls would take.
+struct Arena {
+    char* base; size_t cap, off = 0, peak = 0;
+    bool dry() const { return base == nullptr; }
+    void* take(size_t bytes) {
+        off = (off + 255) & ~(size_t)255;
+        void* p = base ? base + off : nullptr;
+        off += bytes;
+        if (off > peak) peak = off;
+        return p;
+    }
+    bool full() const { return base && peak > cap; }
+};
+
+struct Ctx {
+    Arena& ar; bool bf; hipStream_t st; int rc = ACMIL_OK;
+    bool go() const { return rc == ACMIL_OK && !ar.dry(); }
+    void launched() { if (hipGetLastError() != hipSuccess) rc = ACMIL_ERR_LAUNCH; }
+    bool room() { if (ar.full()) { if (rc == ACMIL_OK) rc = ACMIL_ERR_SHAPE; return false; } return true; }
+};
+
+struct Mat { const void* p; long long ld; int rows, cols; };
+
+inline bool on16(const void* p) { return ((size_t)p & 15) == 0; }
+inline unsigned grid_of(long long items) { const long long g = (items + 255) / 256; return (unsigned)(g < 1 ? 1 : g > 65536 ? 65536 : g); }
+
+// m as the products take it: rows on 16 bytes, a multiple of 8 columns (zeros behind the last)
+Mat aligned(Ctx& c, const Mat& m, bool force = false) {
+    if (!force && on16(m.p) && m.ld % 8 == 0 && m.cols % 8 == 0) return m;
+    const int ldd = r8(m.cols);
+    short* d = (short*)c.ar.take((size_t)m.rows * ldd * 2);
+    if (c.room() && c.go()) {
+        hipLaunchKernelGGL(mm_pad_kernel, dim3(grid_of((long long)m.rows * (ldd / 8))), dim3(256), 0, c.st, (const short*)m.p, m.ld, m.rows, m.cols, d, ldd);
+        c.launched();
+    }
+    return Mat{d, ldd, m.rows, ldd};
+}
+// two matrices that one product addresses with one leading dimension
+void aligned_pair(Ctx& c, Mat& a, Mat& b) {
+    Mat x = aligned(c, a), y = aligned(c, b);
+    if (x.ld != y.ld) {
+        if (x.p == a.p && x.ld != r8(a.cols)) x = aligned(c, a, true);
+        if (y.p == b.p && y.ld != r8(b.cols)) y = aligned(c, b, true);
+    }
+    a = x; b = y;
+}
+
+enum { FWD, DGRAD, WGRAD };
+
+// One product: tile, K split, launch, join.
+void product(Ctx& c, int kind, MmArgs a, int epi) {
+    const bool dual = epi == MM_GATE;
+    const int n_eff = dual ? 2 * a.N : a.N, steps = mm_steps(a);
+    const long long tl = (long long)((a.M + 255) / 256) * ((n_eff + 255) / 256);
+    // 256 x 256 tiles need half the LDS reads and fetches per flop of 128 x 128 ones, but only one fits a CU: taken where they fill
+    // most of the 256 CUs
+    const bool large = tl >= 160;
+    const int b = large ? 256 : 128;
+    a.ntm = (a.M + b - 1) / b;
+    a.ntn = (n_eff + b - 1) / b;
+    const long long tiles = (long long)a.ntm * a.ntn;
+    // few tiles: split K so that the workgroups fill the chip twice over, at least 4 steps each
+    long long sp = large ? 1 : 512 / tiles;
+    if (sp > steps / 4) sp = steps / 4;
+    a.splits = (int)(sp < 1 ? 1 : sp > 64 ? 64 : sp);
+    const size_t mark = c.ar.off;
+    if (a.splits > 1) {
+        a.e.ldpart = r8(a.e.npad);
+        a.e.part = (float*)c.ar.take((size_t)a.splits * (dual ? 2 : 1) * a.M * a.e.ldpart * 4);
+    }
+    if (c.room() && c.go()) {
+        const int e = a.splits > 1 ? MM_PART : epi;
+        c.rc = kind == FWD ? mm_launch_fwd(a, c.bf, e, dual, large, c.st) : kind == DGRAD ? mm_launch_dgrad(a, c.bf, e, large, c.st)
+                                                                             : mm_launch_wgrad(a, c.bf, e, large, c.st);
+        if (a.splits > 1 && c.rc == ACMIL_OK) {
+            const dim3 g((unsigned)(((long long)a.M * (a.e.ldpart / 8) + 255) / 256));
+#define JOIN(B, E) hipLaunchKernelGGL((mm_join_kernel<B, E>), g, dim3(256), 0, c.st, a)
+            if (epi == MM_GATE) { if (c.bf) JOIN(true, MM_GATE); else JOIN(false, MM_GATE); }
+            else if (epi == MM_GATE_BWD) { if (c.bf) JOIN(true, MM_GATE_BWD); else JOIN(false, MM_GATE_BWD); }
+            else { if (c.bf) JOIN(true, MM_ACT); else JOIN(false, MM_ACT); }
+#undef JOIN
+            c.launched();
+        }
+    }
+    c.ar.off = mark;                                                 // the partial sums are dead behind the join: stream order
+}
+
+MmArgs operands(const Mat& q, const Mat& p, int M, int N, int Kq, int Kp) {
+    MmArgs a = {};
+    a.q0 = a.q1 = (const char*)q.p; a.p0 = a.p1 = (const char*)p.p;
+    a.ldq = q.ld * 2; a.ldp = p.ld * 2;
+    a.M = M; a.N = N; a.Kq = Kq; a.Kp = Kp; a.segs = 1; a.splits = 1;
+    a.e.act = ACMIL_ACT_NONE;
+    return a;
+}
+void output(MmArgs& a, void* out, long long ldo, const void* bias = nullptr, const void* res = nullptr, long long ldr = 0) {
+    a.e.out = out; a.e.ldo = ldo; a.e.bias = bias; a.e.res = res; a.e.ldr = ldr; a.e.npad = a.N;
+    a.e.vec = on16(out) && ldo % 8 == 0 && on16(bias) && on16(res) && ldr % 8 == 0;      // null is on 16 bytes
+}
+
+void colsum(Ctx& c, const Mat& x, int rows, int cols, void* out) {
+    const size_t mark = c.ar.off;
+    const int c8 = r8(cols);
+    int gy = rows / 64;
+    gy = gy < 1 ? 1 : gy > 128 ? 128 : gy;
+    float* part = (float*)c.ar.take((size_t)gy * c8 * 4);
+    if (c.room() && c.go()) {
+        const dim3 g((c8 + 255) / 256, gy), j((cols + 255) / 256);
+        if (c.bf) {
+            hipLaunchKernelGGL((mm_colsum_kernel<true>), g, dim3(256), 0, c.st, x.p, x.ld, rows, c8, part);
+            hipLaunchKernelGGL((mm_colsum_join_kernel<true>), j, dim3(256), 0, c.st, part, gy, c8, cols, out);
+        } else {
+            hipLaunchKernelGGL((mm_colsum_kernel<false>), g, dim3(256), 0, c.st, x.p, x.ld, rows, c8, part);
+            hipLaunchKernelGGL((mm_colsum_join_kernel<false>), j, dim3(256), 0, c.st, part, gy, c8, cols, out);
+        }
+        c.launched();
+    }
+    c.ar.off = mark;
+}
+
+// 32-bit byte offsets inside a tile: 256 rows (64 k rows) of the largest leading dimension; 31-bit row and column counts
+const long long MAX_LD = 1LL << 22;
+const int MAX_DIM = 1 << 22;
+
+bool same_dtype_ok(int dtype) { return dtype == ACMIL_DTYPE_F16 || dtype == ACMIL_DTYPE_BF16; }
+bool act_ok(int act) { return act >= ACMIL_ACT_NONE && act <= ACMIL_ACT_SIGMOID; }
+bool ld_ok(const void* p, long long ld, int cols) { return !p || (ld >= 0 && ld <= MAX_LD && (ld >= cols || ld == 0)); }
+
+void few_rows(Ctx& c, const MmArgs& a, bool dual) {
+    if (c.go()) c.rc = mm_launch_rows(a, c.bf, dual, c.st);
+}
+
+int linear_check(const acmil_linear_args* a, bool backward) {
+    if (!a) return ACMIL_ERR_NULL;
+    if (!same_dtype_ok(a->dtype)) return ACMIL_ERR_UNSUPPORTED;
+    if (!act_ok(a->act) || a->M <= 0 || a->K <= 0 || a->N <= 0 || a->K > MAX_DIM || a->N > MAX_DIM) return ACMIL_ERR_SHAPE;
+    if (!a->x || !a->W) return ACMIL_ERR_NULL;
+    if (!ld_ok(a->x, a->ldx, a->K) || !ld_ok(a->W, a->ldw, a->K)) return ACMIL_ERR_SHAPE;
+    if (!backward) {
+        if (!a->y) return ACMIL_ERR_NULL;
+        if (a->ldy < a->N || !ld_ok(a->res, a->ldr, a->N)) return ACMIL_ERR_SHAPE;
+        if (a->pre && !on16(a->pre)) return ACMIL_ERR_SHAPE;
+        return ACMIL_OK;
+    }
+    if (!a->dy || (a->act != ACMIL_ACT_NONE && !a->pre)) return ACMIL_ERR_NULL;
+    if (!ld_ok(a->dy, a->lddy, a->N) || (a->pre && !on16(a->pre))) return ACMIL_ERR_SHAPE;
+    return ACMIL_OK;
+}
+
+int linear_fwd(const acmil_linear_args& a, Ctx& c) {
+    Mat x{a.x, a.ldx, a.M, a.K}, w{a.W, a.ldw, a.N, a.K};
+    const bool few = a.M <= MM_ROWS_MAX;
+    if (!few) { x = aligned(c, x); w = aligned(c, w); }
+    MmArgs p = operands(x, w, a.M, a.N, x.cols, w.cols);
+    output(p, a.y, a.ldy, a.bias, a.res, a.ldr);
+    p.e.act = a.act; p.e.pre = a.pre; p.e.ldp = r8(a.N);
+    if (few) few_rows(c, p, false); else product(c, FWD, p, MM_ACT);
+    return c.rc;
+}
+
+int linear_bwd(const acmil_linear_args& a, Ctx& c) {
+    const Mat dy{a.dy, a.lddy, a.M, a.N};
+    Mat dz;
+    if (a.act == ACMIL_ACT_NONE) dz = aligned(c, dy);
+    else {
+        const int ldz = r8(a.N);
+        void* z = c.ar.take((size_t)a.M * ldz * 2);
+        if (c.room() && c.go()) {
+            const int vec = on16(a.dy) && a.lddy % 8 == 0;
+            const dim3 g(grid_of((long long)a.M * (ldz / 8)));
+            if (c.bf) hipLaunchKernelGGL((mm_dz_kernel<true>), g, dim3(256), 0, c.st, a.dy, a.lddy, vec, a.pre, (long long)ldz, a.act, a.M, a.N, z, ldz);
+            else hipLaunchKernelGGL((mm_dz_kernel<false>), g, dim3(256), 0, c.st, a.dy, a.lddy, vec, a.pre, (long long)ldz, a.act, a.M, a.N, z, ldz);
+            c.launched();
+        }
+        dz = Mat{z, ldz, a.M, ldz};
+    }
+    if (a.dx) {
+        const Mat w = aligned(c, Mat{a.W, a.ldw, a.N, a.K});
+        MmArgs p = operands(dz, w, a.M, a.K, dz.cols, a.N);
+        output(p, a.dx, a.K);
+        product(c, DGRAD, p, MM_ACT);
+    }
+    if (a.dW) {
+        const Mat x = aligned(c, Mat{a.x, a.ldx, a.M, a.K});
+        MmArgs p = operands(dz, x, a.N, a.K, a.M, a.M);
+        output(p, a.dW, a.K);
+        product(c, WGRAD, p, MM_ACT);
+    }
+    if (a.db) colsum(c, dz, a.M, a.N, a.db);
+    return c.rc;
+}
+
+int ffn_check(const acmil_ffn_args* a, bool backward) {
+    if (!a) return ACMIL_ERR_NULL;
+    if (!same_dtype_ok(a->dtype)) return ACMIL_ERR_UNSUPPORTED;
+    if (!act_ok(a->act) || a->M <= 0 || a->D <= 0 || a->F <= 0 || a->D > MAX_DIM || a->F > MAX_DIM / 2) return ACMIL_ERR_SHAPE;
+    if (!a->x || !a->Wg || !a->Wu || !a->Wd) return ACMIL_ERR_NULL;
+    if (!ld_ok(a->x, a->ldx, a->D) || !ld_ok(a->Wg, a->ldwg, a->D) || !ld_ok(a->Wu, a->ldwu, a->D) || !ld_ok(a->Wd, a->ldwd, a->F)) return ACMIL_ERR_SHAPE;
+    const int saved = (a->g != nullptr) + (a->u != nullptr) + (a->h != nullptr);
+    if (saved != 0 && saved != 3) return ACMIL_ERR_NULL;
+    if (!on16(a->g) || !on16(a->u) || !on16(a->h)) return ACMIL_ERR_SHAPE;
+    if (!backward) {
+        if (!a->y) return ACMIL_ERR_NULL;
+        return a->ldy < a->D || !ld_ok(a->res, a->ldr, a->D) ? ACMIL_ERR_SHAPE : ACMIL_OK;
+    }
+    if (!a->dy || saved != 3) return ACMIL_ERR_NULL;
+    return ld_ok(a->dy, a->lddy, a->D) ? ACMIL_OK : ACMIL_ERR_SHAPE;
+}
+
+int ffn_fwd(const acmil_ffn_args& a, Ctx& c) {
+    const int F8 = r8(a.F);
+    const bool few = a.M <= MM_ROWS_MAX;
+    Mat x{a.x, a.ldx, a.M, a.D}, wg{a.Wg, a.ldwg, a.F, a.D}, wu{a.Wu, a.ldwu, a.F, a.D}, wd{a.Wd, a.ldwd, a.D, a.F};
+    if (!few) { x = aligned(c, x); aligned_pair(c, wg, wu); wd = aligned(c, wd); }
+    else if (wg.ld != wu.ld) aligned_pair(c, wg, wu);                // one leading dimension for both
+    Mat h{a.h ? a.h : c.ar.take((size_t)a.M * F8 * 2), F8, a.M, F8};
+    if (!c.room()) return c.rc;
+    MmArgs p = operands(x, wg, a.M, a.F, few ? a.D : x.cols, few ? a.D : wg.cols);
+    p.p1 = (const char*)wu.p;
+    output(p, (void*)h.p, F8, a.bg);
+    p.e.vec = p.e.vec && on16(a.bu);
+    p.e.bias2 = a.bu; p.e.npad = F8; p.e.act = a.act;
+    p.e.pre = a.g; p.e.pre2 = a.u; p.e.ldp = F8;
+    if (few) few_rows(c, p, true); else product(c, FWD, p, MM_GATE);
+    MmArgs d = operands(h, wd, a.M, a.D, few ? a.F : F8, few ? a.F : wd.cols);
+    output(d, a.y, a.ldy, a.bd, a.res, a.ldr);
+    if (few) few_rows(c, d, false); else product(c, FWD, d, MM_ACT);
+    return c.rc;
+}
+
+int ffn_bwd(const acmil_ffn_args& a, Ctx& c) {
+    const int F8 = r8(a.F);
+    const Mat dy = aligned(c, Mat{a.dy, a.lddy, a.M, a.D}), h{a.h, F8, a.M, F8};
+    Mat x{a.x, a.ldx, a.M, a.D};
+    Mat dgu{nullptr, 2LL * F8, a.M, 2 * F8};                         // [dg | du], each with zeros behind column F
+    if (a.dx || a.dWgu || a.dbgu) {
+        const Mat wd = aligned(c, Mat{a.Wd, a.ldwd, a.D, a.F});
+        dgu.p = c.ar.take((size_t)a.M * 2 * F8 * 2);
+        if (!c.room()) return c.rc;
+        MmArgs p = operands(dy, wd, a.M, a.F, dy.cols, a.D);
+        output(p, (void*)dgu.p, 2LL * F8);
+        p.e.out2 = (short*)dgu.p + F8; p.e.npad = F8; p.e.act = a.act;
+        p.e.pre = a.g; p.e.pre2 = a.u; p.e.ldp = F8;
+        product(c, DGRAD, p, MM_GATE_BWD);
+    }
+    if (a.dx) {
+        Mat wg{a.Wg, a.ldwg, a.F, a.D}, wu{a.Wu, a.ldwu, a.F, a.D};
+        aligned_pair(c, wg, wu);
+        MmArgs p = operands(dgu, wg, a.M, a.D, F8, a.F);             // dg Wg + du Wu: two K segments of one product
+        p.segs = 2;
+        p.q1 = p.q0 + 2LL * F8; p.p1 = (const char*)wu.p;
+        output(p, a.dx, a.D);
+        product(c, DGRAD, p, MM_ACT);
+    }
+    if (a.dWgu) {
+        x = aligned(c, x);
+        MmArgs p = operands(dgu, x, 2 * F8, a.D, a.M, a.M);
+        output(p, a.dWgu, a.D);
+        product(c, WGRAD, p, MM_ACT);
+    }
+    if (a.dWd) {
+        MmArgs p = operands(dy, h, a.D, a.F, a.M, a.M);
+        output(p, a.dWd, a.F);
+        product(c, WGRAD, p, MM_ACT);
+    }
+    if (a.dbgu) colsum(c, dgu, a.M, 2 * F8, a.dbgu);
+    if (a.dbd) colsum(c, dy, a.M, a.D, a.dbd);
+    return c.rc;
+}
+
+template <class A> size_t need(const A* a, int rc, int (*f)(const A&, Ctx&)) {
+    if (rc != ACMIL_OK) return 0;
+    Arena ar{nullptr, 0};
+    Ctx c{ar, a->dtype == ACMIL_DTYPE_BF16, nullptr};
+    f(*a, c);
+    return (ar.peak + 255 + 256) & ~(size_t)255;
+}
+template <class A> int go(const A* a, int rc, int (*f)(const A&, Ctx&), void* ws, size_t bytes, void* stream) {
+    if (rc != ACMIL_OK) return rc;
+    if (!ws) return ACMIL_ERR_NULL;
+    if (((size_t)ws & 255) != 0) return ACMIL_ERR_SHAPE;
+    if (bytes < need(a, rc, f)) return ACMIL_ERR_SHAPE;              // before anything is launched
+    Arena ar{(char*)ws, bytes};
+    Ctx c{ar, a->dtype == ACMIL_DTYPE_BF16, (hipStream_t)stream};
+    return f(*a, c);
+}
+
+}  // namespace
+
+extern "C" size_t acmil_linear_act_workspace_bytes(const acmil_linear_args* a) { return need(a, linear_check(a, false), linear_fwd); }
+extern "C" int acmil_linear_act(const acmil_linear_args* a, void* workspace, size_t workspace_bytes, void* stream) {
+    return go(a, linear_check(a, false), linear_fwd, workspace, workspace_bytes, stream);
+}
+extern "C" size_t acmil_linear_act_bwd_workspace_bytes(const acmil_linear_args* a) { return need(a, linear_check(a, true), linear_bwd); }
+extern "C" int acmil_linear_act_bwd(const acmil_linear_args* a, void* workspace, size_t workspace_bytes, void* stream) {
+    return go(a, linear_check(a, true), linear_bwd, workspace, workspace_bytes, stream);
+}
+extern "C" size_t acmil_gated_ffn_workspace_bytes(const acmil_ffn_args* a) { return need(a, ffn_check(a, false), ffn_fwd); }
+extern "C" int acmil_gated_ffn(const acmil_ffn_args* a, void* workspace, size_t workspace_bytes, void* stream) {
+    return go(a, ffn_check(a, false), ffn_fwd, workspace, workspace_bytes, stream);
+}
+extern "C" size_t acmil_gated_ffn_bwd_workspace_bytes(const acmil_ffn_args* a) { return need(a, ffn_check(a, true), ffn_bwd); }
+extern "C" int acmil_gated_ffn_bwd(const acmil_ffn_args* a, void* workspace, size_t workspace_bytes, void* stream) {
+    return go(a, ffn_check(a, true), ffn_bwd, workspace, workspace_bytes, stream);
+}

@@ -952,3 +952,200 @@ def linear_f16x3(x: torch.Tensor, packed: torch.Tensor, n_out: int, bias: Option
     _lib.check(rc, "acmil_linear_f16x3")
     return (out, ws[8:12].view(torch.int32)) if want_status else out
 
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# 16-bit linear layer with a fused epilogue, gated feed-forward block (csrc/mm16*.hip)
+# ---------------------------------------------------------------------------------------------------------------------
+_HALF = (torch.float16, torch.bfloat16)
+_MAX_ROWS, _MAX_DIM, _MAX_LD = (1 << 31) - 1, 1 << 22, 1 << 22
+
+
+def _half_inputs(name: str, *ts: Optional[torch.Tensor]) -> torch.device:
+    """One CUDA device and one 16-bit type for every tensor of the call."""
+    _need_cuda(*ts)
+    first = ts[0]
+    if first.dtype not in _HALF:
+        raise RuntimeError("acmil_amd.%s: fp16 or bf16 tensors (got %s); fp32 layers are acmil_amd.autograd.linear / ops.linear_f16x3" % (name, first.dtype))
+    for t in ts:
+        if t is not None and (t.dtype != first.dtype or t.device != first.device):
+            raise RuntimeError("acmil_amd.%s: all tensors must have one type and one device (%s on %s and %s on %s)"
+                               % (name, first.dtype, first.device, t.dtype, t.device))
+    return first.device
+
+
+def _act_id(name: str, act: str) -> int:
+    if act not in _lib.ACTS:
+        raise ValueError("acmil_amd.%s: act must be one of %s, got %r" % (name, ", ".join(_lib.ACTS), act))
+    return _lib.ACTS[act]
+
+
+def _rows16(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
+    """t [..., C] as a matrix the library can address: (2-D tensor with unit inner stride, leading dimension).  Row strides are kept
+    (0 = every row the same); anything else -- a strided inner dimension, overlapping rows -- is copied once."""
+    t = t.detach()
+    c = t.shape[-1]
+    if t.dim() != 2:
+        t = t.reshape(-1, c)
+    ld = t.stride(0) if t.shape[0] > 1 else c
+    if (c > 1 and t.stride(1) != 1) or (ld != 0 and ld < c) or ld > _MAX_LD:
+        t = t.contiguous()
+        ld = c
+    return t, ld
+
+
+def _vec16(name: str, what: str, t: Optional[torch.Tensor], n: int) -> Optional[torch.Tensor]:
+    if t is None:
+        return None
+    if t.shape != (n,):
+        raise RuntimeError("acmil_amd.%s: %s must be [%d], got %s" % (name, what, n, tuple(t.shape)))
+    return t.detach().contiguous()
+
+
+def _half_call(name: str, args, device: torch.device) -> None:
+    """Workspace query + call of a C entry that takes one argument block, on the tensors' device and its current stream."""
+    lib = _lib.load()
+    if device.index is not None and device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _half_call(name, args, device)
+    ref = ctypes.byref(args)
+    need = getattr(lib, name + "_workspace_bytes")(ref)
+    if need == 0:
+        raise RuntimeError("%s: the arguments are refused (a dimension or leading dimension is out of range)" % name)
+    ws = torch.empty(need, dtype=torch.uint8, device=device)
+    _lib.check(getattr(lib, name)(ref, ws.data_ptr(), need, _stream()), name)
+
+
+def _linear_args(name: str, x: torch.Tensor, weight: torch.Tensor, act: str):
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or 0 in weight.shape:
+        raise RuntimeError("acmil_amd.%s: x [..., in] and weight [out, in] expected, got %s and %s" % (name, tuple(x.shape), tuple(weight.shape)))
+    if max(weight.shape) > _MAX_DIM or x.numel() // weight.shape[1] > _MAX_ROWS:
+        raise RuntimeError("acmil_amd.%s: at most %d features and %d rows" % (name, _MAX_DIM, _MAX_ROWS))
+    a = _lib.LinearArgs(dtype=_DT[x.dtype], act=_act_id(name, act))
+    x2, a.ldx = _rows16(x)
+    w2, a.ldw = _rows16(weight)
+    a.M, a.K, a.N = x2.shape[0], x2.shape[1], w2.shape[0]
+    a.x, a.W = x2.data_ptr(), w2.data_ptr()
+    return a, x2, w2
+
+
+def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, act: str = "none",
+               residual: Optional[torch.Tensor] = None, keep_pre: bool = False):
+    """acmil_linear_act: y = act(x @ weight^T + bias) + residual in ONE launch of the product (fp16 or bf16; fp32 accumulation and
+    epilogue, one rounding at the end).  x [..., in], weight [out, in], bias [out], residual [..., out]; act one of none, relu, silu, gelu,
+    gelu_tanh, sigmoid.  Any row strides and sizes; no rows give an empty result.  keep_pre: also x @ weight^T + bias in fp32
+    ([rows, round8(out)]), what linear_act_bwd wants.  No gradient is recorded (acmil_amd.autograd.linear_act is the differentiable form)."""
+    dev = _half_inputs("linear_act", x, weight, bias, residual)
+    a, x2, w2 = _linear_args("linear_act", x, weight, act)
+    shape = tuple(x.shape[:-1]) + (a.N,)
+    b = _vec16("linear_act", "bias", bias, a.N)
+    if residual is not None and tuple(residual.shape) != shape:
+        raise RuntimeError("acmil_amd.linear_act: residual must be %s, got %s" % (shape, tuple(residual.shape)))
+    y = torch.empty(shape, dtype=x.dtype, device=dev)
+    pre = torch.empty(a.M, (a.N + 7) // 8 * 8, dtype=torch.float32, device=dev) if keep_pre else None
+    if a.M > 0:
+        a.y, a.ldy, a.bias, a.pre = y.data_ptr(), a.N, _ptr(b), _ptr(pre)
+        r2 = None
+        if residual is not None:
+            r2, a.ldr = _rows16(residual)
+            a.res = r2.data_ptr()
+        _half_call("acmil_linear_act", a, dev)
+    return (y, pre) if keep_pre else y
+
+
+def linear_act_bwd(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, pre: Optional[torch.Tensor] = None, act: str = "none",
+                   need: Sequence[bool] = (True, True, True)):
+    """acmil_linear_act_bwd: (dx, dweight, dbias) of linear_act for the incoming dy [..., out] and the kept `pre` (act "none" needs none);
+    need = which of the three to form (None in the others' places).  The residual's gradient is dy."""
+    dev = _half_inputs("linear_act_bwd", x, weight, dy)
+    a, x2, w2 = _linear_args("linear_act_bwd", x, weight, act)
+    if tuple(dy.shape) != tuple(x.shape[:-1]) + (a.N,):
+        raise RuntimeError("acmil_amd.linear_act_bwd: dy must be %s, got %s" % (tuple(x.shape[:-1]) + (a.N,), tuple(dy.shape)))
+    if act != "none" and (pre is None or pre.dtype != torch.float32 or pre.device != dev or not pre.is_contiguous()
+                          or tuple(pre.shape) != (a.M, (a.N + 7) // 8 * 8)):
+        raise RuntimeError("acmil_amd.linear_act_bwd: act %r needs the pre-activations linear_act(keep_pre=True) returned" % act)
+    make = torch.empty if a.M > 0 else torch.zeros
+    dx = make(x.shape, dtype=x.dtype, device=dev) if need[0] else None
+    dw = make(weight.shape, dtype=x.dtype, device=dev) if need[1] else None
+    db = make(a.N, dtype=x.dtype, device=dev) if need[2] else None
+    if a.M > 0 and any(need):
+        dy2, a.lddy = _rows16(dy)
+        a.dy, a.pre, a.dx, a.dW, a.db = dy2.data_ptr(), _ptr(pre), _ptr(dx), _ptr(dw), _ptr(db)
+        _half_call("acmil_linear_act_bwd", a, dev)
+    return dx, dw, db
+
+
+def _ffn_args(name: str, x, w_gate, w_up, w_down, act: str):
+    if (w_gate.dim() != 2 or x.dim() < 1 or x.shape[-1] != w_gate.shape[1] or w_up.shape != w_gate.shape
+            or tuple(w_down.shape) != (w_gate.shape[1], w_gate.shape[0]) or 0 in w_gate.shape):
+        raise RuntimeError("acmil_amd.%s: x [..., D], w_gate and w_up [F, D], w_down [D, F] expected, got %s, %s, %s, %s"
+                           % (name, tuple(x.shape), tuple(w_gate.shape), tuple(w_up.shape), tuple(w_down.shape)))
+    F, D = w_gate.shape
+    if D > _MAX_DIM or F > _MAX_DIM // 2 or x.numel() // D > _MAX_ROWS:
+        raise RuntimeError("acmil_amd.%s: at most %d features, %d hidden features and %d rows" % (name, _MAX_DIM, _MAX_DIM // 2, _MAX_ROWS))
+    a = _lib.FfnArgs(dtype=_DT[x.dtype], act=_act_id(name, act), D=D, F=F)
+    x2, a.ldx = _rows16(x)
+    g2, a.ldwg = _rows16(w_gate)
+    u2, a.ldwu = _rows16(w_up)
+    d2, a.ldwd = _rows16(w_down)
+    a.M, a.x, a.Wg, a.Wu, a.Wd = x2.shape[0], x2.data_ptr(), g2.data_ptr(), u2.data_ptr(), d2.data_ptr()
+    return a, (x2, g2, u2, d2)
+
+
+def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, b_gate: Optional[torch.Tensor] = None,
+              b_up: Optional[torch.Tensor] = None, b_down: Optional[torch.Tensor] = None, act: str = "silu",
+              residual: Optional[torch.Tensor] = None, keep: bool = False):
+    """acmil_gated_ffn: y = (act(x @ w_gate^T + b_gate) * (x @ w_up^T + b_up)) @ w_down^T + b_down + residual, fp16 or bf16, two launches:
+    both projections, the activation and the product in one, the projection back with bias and residual in the other.  x [..., D], w_gate and
+    w_up [F, D], w_down [D, F], residual [..., D]; act as linear_act ("silu" is the SwiGLU block, "gelu" GeGLU, "sigmoid" GLU, ...).
+    The gated features between the launches are held in x's type.  keep: also (g, u, h) for gated_ffn_bwd (g, u fp32 and h, each
+    [rows, round8(F)]).  No gradient is recorded (acmil_amd.autograd.gated_ffn is the differentiable form)."""
+    dev = _half_inputs("gated_ffn", x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual)
+    a, hold = _ffn_args("gated_ffn", x, w_gate, w_up, w_down, act)
+    bg, bu, bd = _vec16("gated_ffn", "b_gate", b_gate, a.F), _vec16("gated_ffn", "b_up", b_up, a.F), _vec16("gated_ffn", "b_down", b_down, a.D)
+    if residual is not None and residual.shape != x.shape:
+        raise RuntimeError("acmil_amd.gated_ffn: residual must be %s, got %s" % (tuple(x.shape), tuple(residual.shape)))
+    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    saved = None
+    if keep:
+        f8 = (a.F + 7) // 8 * 8
+        saved = (torch.empty(a.M, f8, dtype=torch.float32, device=dev), torch.empty(a.M, f8, dtype=torch.float32, device=dev),
+                 torch.empty(a.M, f8, dtype=x.dtype, device=dev))
+        a.g, a.u, a.h = (t.data_ptr() for t in saved)
+    if a.M > 0:
+        a.y, a.ldy, a.bg, a.bu, a.bd = y.data_ptr(), a.D, _ptr(bg), _ptr(bu), _ptr(bd)
+        if residual is not None:
+            r2, a.ldr = _rows16(residual)
+            a.res = r2.data_ptr()
+        _half_call("acmil_gated_ffn", a, dev)
+    return (y, saved) if keep else y
+
+
+def gated_ffn_bwd(dy: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, saved,
+                  act: str = "silu", need_x: bool = True, need_gate_up: bool = True, need_down: bool = True, need_gate_up_bias: bool = False,
+                  need_down_bias: bool = False):
+    """acmil_gated_ffn_bwd: (dx, dw_gate, dw_up, dw_down, db_gate, db_up, db_down) of gated_ffn for the incoming dy [..., D] and what
+    gated_ffn(keep=True) kept; None where not asked for.  dw_gate / dw_up and db_gate / db_up are views of one buffer each.  The residual's gradient is dy."""
+    dev = _half_inputs("gated_ffn_bwd", x, w_gate, w_up, w_down, dy)
+    a, hold = _ffn_args("gated_ffn_bwd", x, w_gate, w_up, w_down, act)
+    if dy.shape != x.shape:
+        raise RuntimeError("acmil_amd.gated_ffn_bwd: dy must be %s, got %s" % (tuple(x.shape), tuple(dy.shape)))
+    f8 = (a.F + 7) // 8 * 8
+    g, u, h = saved
+    for t, dt in ((g, torch.float32), (u, torch.float32), (h, x.dtype)):
+        if t.dtype != dt or t.device != dev or not t.is_contiguous() or tuple(t.shape) != (a.M, f8):
+            raise RuntimeError("acmil_amd.gated_ffn_bwd: saved must be what gated_ffn(keep=True) returned for this x")
+    make = torch.empty if a.M > 0 else torch.zeros
+    dx = make(x.shape, dtype=x.dtype, device=dev) if need_x else None
+    dgu = make(2 * f8, a.D, dtype=x.dtype, device=dev) if need_gate_up else None
+    dd = make(a.D, a.F, dtype=x.dtype, device=dev) if need_down else None
+    bgu = make(2 * f8, dtype=x.dtype, device=dev) if need_gate_up_bias else None
+    bd = make(a.D, dtype=x.dtype, device=dev) if need_down_bias else None
+    if a.M > 0:
+        dy2, a.lddy = _rows16(dy)
+        a.dy, a.g, a.u, a.h = dy2.data_ptr(), g.data_ptr(), u.data_ptr(), h.data_ptr()
+        a.dx, a.dWgu, a.dWd, a.dbgu, a.dbd = _ptr(dx), _ptr(dgu), _ptr(dd), _ptr(bgu), _ptr(bd)
+        _half_call("acmil_gated_ffn_bwd", a, dev)
+    F = a.F
+    return (dx, None if dgu is None else dgu[:F], None if dgu is None else dgu[f8:f8 + F], dd,
+            None if bgu is None else bgu[:F], None if bgu is None else bgu[f8:f8 + F], bd)

@@ -592,6 +592,70 @@ int acmil_adamw_step_peer(float* params, float* exp_avg, float* exp_avg_sq, long
                           double beta1, double beta2, float eps, float weight_decay, long long launch, int use_flag, int* skipped,
                           float* flag_report, float* reduced_out, void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * 16-bit linear layer with a fused epilogue, and the gated feed-forward block (csrc/mm16*.hip).  The reference trains and serves in
+ * fp32 only (architecture/network.py:22-57 holds its linear and residual layers); these are the 16-bit forms for wider models.
+ * All tensors of one call have ONE type (dtype: ACMIL_DTYPE_F16 / _BF16); products accumulate in fp32, bias, activation, gate and
+ * residual are applied in fp32, and every output is rounded once.  Matrices are row-major with unit inner stride; a leading dimension
+ * (in elements) may exceed the row, or be 0 (every row the same); base addresses need 2-byte alignment only.  Matrices whose rows do
+ * not start on 16 bytes or whose length is no multiple of 8 are copied into the workspace first, except in calls of at most 32 rows.
+ *   acmil_linear_act      y [M,N] = act(x W^T + bias) + res        x [M,K], W [N,K], bias [N] or NULL, res [M,N] or NULL (ldr)
+ *     pre: NULL, or fp32 [M][round8(N)] (16-byte aligned) that receives x W^T + bias for the backward (act != NONE needs it)
+ *   acmil_linear_act_bwd  dz = dy act'(pre); dx [M,K] = dz W, dW [N,K] = dz^T x, db [N] = column sums of dz (each may be NULL; dense);
+ *     dz is held in the tensors' type.  The gradient of res is dy itself.
+ *   acmil_gated_ffn       h = act(x Wg^T + bg) * (x Wu^T + bu);  y [M,D] = h Wd^T + bd + res    x [M,D], Wg, Wu [F,D], Wd [D,F]
+ *     h is held in the tensors' type.  g, u (fp32 [M][round8(F)]) and h ([M][round8(F)] of dtype), 16-byte aligned: kept for the
+ *     backward, all three or none (h then lives in the workspace).
+ *   acmil_gated_ffn_bwd   dh = dy Wd, dg = dh u act'(g), du = dh act(g) (both held in the tensors' type);
+ *     dx = dg Wg + du Wu; dWgu [2 round8(F)][D]: rows 0.. = dg^T x, rows round8(F).. = du^T x; dWd [D,F] = dy^T h;
+ *     dbgu [2 round8(F)]: dbg, dbu likewise; dbd [D]  (each may be NULL; dense)
+ * Results are reproducible bit for bit (no atomics; K splits are joined in a fixed order).
+ * workspace: acmil_*_workspace_bytes(args) bytes, 256-byte aligned, contents arbitrary, dead when the call's work is done.  The
+ * query reads the same argument block (base addresses included: they decide about copies); 0 = the arguments are refused.
+ * 1 <= M; 1 <= K, N, D <= 2^22, F <= 2^21; leading dimensions <= 2^22.
+ * ------------------------------------------------------------------------------------------- */
+#define ACMIL_ACT_NONE 0
+#define ACMIL_ACT_RELU 1
+#define ACMIL_ACT_SILU 2      /* z sigmoid(z) */
+#define ACMIL_ACT_GELU 3      /* z Phi(z) */
+#define ACMIL_ACT_GELU_TANH 4 /* 0.5 z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) */
+#define ACMIL_ACT_SIGMOID 5
+
+typedef struct acmil_linear_args {
+    int dtype, act, M, K, N;
+    const void* x; long long ldx;
+    const void* W; long long ldw;
+    const void* bias;
+    const void* res; long long ldr;
+    void* y; long long ldy;
+    float* pre;
+    const void* dy; long long lddy;   /* backward from here on */
+    void *dx, *dW, *db;
+} acmil_linear_args;
+
+typedef struct acmil_ffn_args {
+    int dtype, act, M, D, F;
+    const void* x; long long ldx;
+    const void* Wg; long long ldwg;
+    const void* Wu; long long ldwu;
+    const void* Wd; long long ldwd;
+    const void *bg, *bu, *bd;
+    const void* res; long long ldr;
+    void* y; long long ldy;
+    float *g, *u; void* h;
+    const void* dy; long long lddy;   /* backward from here on */
+    void *dx, *dWgu, *dWd, *dbgu, *dbd;
+} acmil_ffn_args;
+
+size_t acmil_linear_act_workspace_bytes(const acmil_linear_args* args);
+int acmil_linear_act(const acmil_linear_args* args, void* workspace, size_t workspace_bytes, void* stream);
+size_t acmil_linear_act_bwd_workspace_bytes(const acmil_linear_args* args);
+int acmil_linear_act_bwd(const acmil_linear_args* args, void* workspace, size_t workspace_bytes, void* stream);
+size_t acmil_gated_ffn_workspace_bytes(const acmil_ffn_args* args);
+int acmil_gated_ffn(const acmil_ffn_args* args, void* workspace, size_t workspace_bytes, void* stream);
+size_t acmil_gated_ffn_bwd_workspace_bytes(const acmil_ffn_args* args);
+int acmil_gated_ffn_bwd(const acmil_ffn_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

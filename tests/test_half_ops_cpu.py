@@ -1,0 +1,89 @@
+"""16-bit linear layer, gated block: what they refuse, on the CPU (nothing reaches a kernel), and the reference's own gradients."""
+import ctypes
+
+import pytest
+import torch
+
+import half_reference as R
+from acmil_amd import _lib, autograd, ops
+
+
+def test_cpu_tensors_and_other_types_are_refused():
+    x, w = torch.zeros(4, 16, dtype=torch.float16), torch.zeros(8, 16, dtype=torch.float16)
+    for call in (lambda: ops.linear_act(x, w), lambda: autograd.linear_act(x, w), lambda: ops.gated_ffn(x, w, w, w.t()),
+                 lambda: autograd.gated_ffn(x, w, w, w.t())):
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            call()
+
+
+@pytest.mark.parametrize("change, code", [
+    ({}, -3), ({"dtype": 0}, -2), ({"dtype": 7}, -2), ({"act": 9}, -1), ({"M": 0}, -1), ({"K": 0}, -1), ({"N": -1}, -1), ({"K": (1 << 22) + 1}, -1),
+    ({"x": 4096, "W": 4096, "ldx": 15, "ldw": 16}, -1), ({"x": 4096, "W": 4096, "ldx": 16, "ldw": 1 << 23}, -1), ({"x": 4096, "W": 4096, "ldx": 16, "ldw": 16}, -3),
+    ({"x": 4096, "W": 4096, "ldx": 16, "ldw": 16, "y": 4096, "ldy": 7}, -1),
+    ({"x": 4096, "W": 4096, "ldx": 16, "ldw": 16, "y": 4096, "ldy": 8, "pre": 4100}, -1),
+    ({"x": 4096, "W": 4096, "ldx": 16, "ldw": 16, "y": 4096, "ldy": 8, "res": 4096, "ldr": 3}, -1)])
+def test_linear_entry_refuses(change, code):
+    """error codes before anything is launched; the workspace query answers 0 for the same block"""
+    lib = _lib.load()
+    a = _lib.LinearArgs(**{**dict(dtype=1, act=0, M=4, K=16, N=8), **change})
+    assert lib.acmil_linear_act(ctypes.byref(a), None, 0, None) == code
+    assert lib.acmil_linear_act_workspace_bytes(ctypes.byref(a)) == 0
+
+
+def test_entries_refuse_missing_pieces():
+    lib = _lib.load()
+    good = dict(dtype=2, act=2, M=40, K=16, N=8, x=4096, W=4096, ldx=16, ldw=16, y=4096, ldy=8)
+    a = _lib.LinearArgs(**good)
+    need = lib.acmil_linear_act_workspace_bytes(ctypes.byref(a))
+    assert need >= 256
+    assert lib.acmil_linear_act(ctypes.byref(a), None, need, None) == -3                 # no workspace
+    assert lib.acmil_linear_act(ctypes.byref(a), 4097, need, None) == -1                 # not on 256 bytes
+    assert lib.acmil_linear_act(ctypes.byref(a), 4096, need - 1, None) == -1             # too small
+    assert lib.acmil_linear_act(None, 4096, need, None) == -3
+    assert lib.acmil_linear_act_bwd(ctypes.byref(a), 4096, 1 << 30, None) == -3          # no dy
+    b = _lib.LinearArgs(**good, dy=4096, lddy=8)
+    assert lib.acmil_linear_act_bwd(ctypes.byref(b), 4096, 1 << 30, None) == -3          # an activation, but no pre
+    f = dict(dtype=1, act=2, M=40, D=16, F=24, x=4096, ldx=16, Wg=4096, ldwg=16, Wu=4096, ldwu=16, Wd=4096, ldwd=24, y=4096, ldy=16)
+    assert lib.acmil_gated_ffn_workspace_bytes(ctypes.byref(_lib.FfnArgs(**f))) > 0
+    for change, code in (({"Wu": None}, -3), ({"ldwd": 23}, -1), ({"g": 4096}, -3), ({"g": 4096, "u": 4096, "h": 4098}, -1), ({"y": None}, -3),
+                         ({"F": (1 << 21) + 1, "ldwd": 1 << 22}, -1), ({"act": -1}, -1), ({"dtype": 0}, -2)):
+        a = _lib.FfnArgs(**{**f, **change})
+        assert lib.acmil_gated_ffn(ctypes.byref(a), 4096, 1 << 30, None) == code, change
+    a = _lib.FfnArgs(**f, dy=4096, lddy=16)
+    assert lib.acmil_gated_ffn_bwd(ctypes.byref(a), 4096, 1 << 30, None) == -3           # nothing kept by the forward
+
+
+def test_workspace_grows_only_with_copies_and_splits():
+    """rows that lie on 16 bytes need no copy; a shifted base address or an odd length does"""
+    lib = _lib.load()
+    base = dict(dtype=1, act=0, M=4096, K=1024, N=4096, ldx=1024, ldw=1024, y=4096, ldy=4096, W=1 << 20)
+    assert lib.acmil_linear_act_workspace_bytes(ctypes.byref(_lib.LinearArgs(**base, x=1 << 20))) <= 512
+    assert lib.acmil_linear_act_workspace_bytes(ctypes.byref(_lib.LinearArgs(**base, x=(1 << 20) + 2))) >= 4096 * 1024 * 2
+    assert lib.acmil_linear_act_workspace_bytes(ctypes.byref(_lib.LinearArgs(**{**base, "M": 32}, x=(1 << 20) + 2))) <= 512
+
+
+@pytest.mark.parametrize("act", list(_lib.ACTS))
+def test_reference_gradients_are_those_of_differences(act):
+    """the 64-bit reference the GPU tests trust: its gradients against central differences and autograd"""
+    g = torch.Generator().manual_seed(3)
+    x, w, b, r, dy = (torch.randn(*s, generator=g) for s in ((5, 6), (7, 6), (7,), (5, 7), (5, 7)))
+    x, w, b, r, dy = (t.to(torch.bfloat16) for t in (x, w, b, r, dy))
+    ref = R.linear_ref(x, w, b, act, r, dy)
+    h = 1e-6
+    for name, t, d in (("dx", x, 0), ("dw", w, 1), ("db", b, 2)):
+        args = [x.double(), w.double(), b.double()]
+        num = torch.zeros(t.shape, dtype=torch.float64)
+        for i in range(t.numel()):
+            hi, lo = [a.clone() for a in args], [a.clone() for a in args]
+            hi[d].view(-1)[i] += h
+            lo[d].view(-1)[i] -= h
+            f = lambda a: (R.act64(act, a[0] @ a[1].t() + a[2])[0] * dy.double()).sum()
+            num.view(-1)[i] = (f(hi) - f(lo)) / (2 * h)
+        assert (ref[name].v - num).abs().max() < 1e-7 * (1 + num.abs().max())
+    xs = [t.double().requires_grad_() for t in (x, w, w * 0.5, w.t().contiguous())]
+    a, _ = R.act64(act, xs[0] @ xs[1].t())
+    y = (a * (xs[0] @ xs[2].t())) @ xs[3].t()
+    grads = torch.autograd.grad(y, xs, x.double())
+    ref = R.ffn_ref(x, w, w * 0.5, w.t().contiguous(), None, None, None, act, None, x)
+    for k, t in zip(("dx", "dwg", "dwu", "dwd"), grads):
+        assert (ref[k].v - t).abs().max() < 1e-9 * (1 + t.abs().max()), k
