@@ -131,6 +131,8 @@ SIGNATURES = {
     "acmil_gated_ffn": (_i, [_vp, _vp, _sz, _vp]),
     "acmil_gated_ffn_bwd_workspace_bytes": (_sz, [_vp]),
     "acmil_gated_ffn_bwd": (_i, [_vp, _vp, _sz, _vp]),
+    "acmil_orthogonalize_workspace_bytes": (_sz, [_i, _vp, _i]),
+    "acmil_orthogonalize": (_i, [_i, _vp, _i, _i, C.POINTER(C.c_float), C.c_float, _vp, _sz, _vp]),
 }
 
 
@@ -158,6 +160,11 @@ class FfnArgs(C.Structure):
                 ("Wu", _vp), ("ldwu", _ll), ("Wd", _vp), ("ldwd", _ll), ("bg", _vp), ("bu", _vp), ("bd", _vp), ("res", _vp), ("ldr", _ll),
                 ("y", _vp), ("ldy", _ll), ("g", _vp), ("u", _vp), ("h", _vp), ("dy", _vp), ("lddy", _ll), ("dx", _vp), ("dWgu", _vp),
                 ("dWd", _vp), ("dbgu", _vp), ("dbd", _vp)]
+
+
+class OrthoMat(C.Structure):
+    """struct acmil_ortho_mat (include/acmil_hip.h)"""
+    _fields_ = [("g", _vp), ("ldg", _ll), ("o", _vp), ("ldo", _ll), ("m", _i), ("n", _i)]
 
 
 _lib = None

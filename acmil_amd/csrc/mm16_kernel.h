@@ -22,13 +22,16 @@ typedef __attribute__((address_space(3))) char mm_lds;
 
 static __device__ __attribute__((aligned(16))) unsigned mm_zero[4];     // what a lane fetches in place of a chunk beyond K
 
-// tile geometry: L = one 8-wave workgroup per CU (128 KB of LDS), S = two 4-wave workgroups per CU
-template <bool LARGE> struct MmCfg {
-    static constexpr int BM = LARGE ? 256 : 128, BN = LARGE ? 256 : 128, WAVES = LARGE ? 8 : 4;
-    static constexpr int WN = LARGE ? 4 : 2;                        // waves along the columns; each owns 64 of them
-    static constexpr int TM = BM / (WAVES / WN), MT = TM / 32;      // rows of a wave, in 32-row tiles
+// tile geometry: WAVES waves, WN of them along the columns, each with MT x NT accumulator tiles of 32 x 32
+template <int BM_, int BN_, int WAVES_, int WN_> struct MmGeom {
+    static constexpr int BM = BM_, BN = BN_, WAVES = WAVES_, WN = WN_;
+    static constexpr int TM = BM / (WAVES / WN), TN = BN / WN, MT = TM / 32, NT = TN / 32;
     static constexpr int QB = BM * 128, PB = BN * 128, STAGE = QB + PB;
 };
+// LARGE: one 8-wave workgroup per CU (128 KB of LDS), else two 4-wave workgroups per CU
+template <bool LARGE> struct MmCfg;
+template <> struct MmCfg<true> : MmGeom<256, 256, 8, 4> {};
+template <> struct MmCfg<false> : MmGeom<128, 128, 4, 2> {};
 
 __device__ __forceinline__ unsigned mm_lds_addr(const void* p) { return (unsigned)(size_t)(const __attribute__((address_space(3))) void*)p; }
 
@@ -113,7 +116,7 @@ template <bool BF> __device__ __forceinline__ f32x16 mm_mfma(s16x8 a, s16x8 b, f
 template <bool BF, int PK, int QK, int EPI, bool DUAL, bool LARGE>
 __global__ __launch_bounds__(MmCfg<LARGE>::WAVES * 64, 2) void mm16_kernel(MmArgs a) {
     using C = MmCfg<LARGE>;
-    constexpr int MT = C::MT, NT = 2;
+    constexpr int MT = C::MT, NT = C::NT;
     __shared__ __attribute__((aligned(128))) char smem[2 * C::STAGE];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / C::WN, wn = wave % C::WN;

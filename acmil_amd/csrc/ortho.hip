@@ -1,0 +1,444 @@
+// ortho.hip -- orthogonalisation of matrices by Newton-Schulz products: X = G / (|G|_F + eps), then `steps` times
+//   A = X X^T;   B = b A + c A A;   X <- a X + B X        (on G^T where G has more rows than columns, so that A is the small Gram matrix).
+// The odd polynomial a s + b s^3 + c s^5 acts on the singular values and drives them towards 1, whatever the singular vectors are.
+//
+// Arithmetic.  A single 16-bit product would not do: errors of the null directions are multiplied by a^steps (485 for 3.4445^5).  Every
+// value is held as a pair of f16 halves, hi + lo (22 bits and a common power-of-two scale, so that nothing is lost to the narrow
+// exponent: |X|, |A|, |B| are bounded by the polynomial, checked on the host), and a product is hi hi + hi lo + lo hi on
+// v_mfma_f32_32x32x16_f16 with fp32 accumulation -- as exact as an fp32 product at a multiple of its rate.
+//
+// Layout.  A row of K values lies as blocks of 32: 64 bytes of hi halves, then 64 bytes of lo halves.  A K step of 32 is then
+// exactly one 128-byte row piece, and tiles move and lie in LDS like those of mm16_kernel.h; of a fragment's four 16-wide pieces two
+// are hi and two lo.  K is padded to a multiple of 32 with zeros, so there is no tail.  All three products take both operands with K
+// contiguous: X is kept in both orientations (its transpose twice, read and written alternately).  A and B are symmetric: only tiles on
+// and below the diagonal are computed and each is written a second time, mirrored.
+// All matrices of a call go through the same launches: 2 + 3 steps of them, whatever the number of matrices (up to NS_GROUP at a time).
+#include "mm16_kernel.h"
+
+#include <cmath>
+
+#define NS_GROUP 24
+#define NS_SCALE 4096.0f          // |X| <= 3.9, |A|, |B| <= 15.5 (host check) stay below 65504
+
+struct NsMat {
+    const void* g; void* o; long long ldg, ldo;
+    char *X, *XT0, *XT1, *A, *B;  // pair planes: X [s][t], XT [t][s], A and B [s][s]
+    int s, t, tall, pad;          // s <= t; tall: G is [t][s]
+};
+struct NsArgs {
+    int count, flip, last;        // flip: XT1 is the present transpose; last: X goes to o
+    float a, b, c;
+    float eps;
+    const double* part; int nparts;
+    int first[NS_GROUP + 1];      // first workgroup of each matrix
+    NsMat m[NS_GROUP];
+};
+
+enum { NS_GRAM = 0, NS_POLY = 1, NS_STEP = 2 };
+
+__host__ __device__ static inline int ns_r32(int n) { return (n + 31) & ~31; }
+__host__ __device__ static inline long long ns_ld(int k) { return ns_r32(k) * 4LL; }           // bytes of a row of k pairs
+__device__ __forceinline__ long long ns_at(int k) { return (k >> 5) * 128LL + (k & 31) * 2; }  // byte of the hi half of column k; lo: + 64
+
+__device__ __forceinline__ int ns_find(const NsArgs& a, int b) {
+    int i = 0;
+    while (i + 1 < a.count && b >= a.first[i + 1]) ++i;
+    return i;
+}
+
+template <int DT> __device__ __forceinline__ float ns_load(const void* p, long long i) {
+    if constexpr (DT == ACMIL_DTYPE_F32) return ((const float*)p)[i];
+    else if constexpr (DT == ACMIL_DTYPE_F16) return (float)((const _Float16*)p)[i];
+    else return (float)((const __bf16*)p)[i];
+}
+template <int DT> __device__ __forceinline__ void ns_store(void* p, long long i, float v) {
+    if constexpr (DT == ACMIL_DTYPE_F32) ((float*)p)[i] = v;
+    else if constexpr (DT == ACMIL_DTYPE_F16) ((_Float16*)p)[i] = (_Float16)v;
+    else ((__bf16*)p)[i] = (__bf16)v;
+}
+
+// sum of squares, in 64 bits (a gradient's squares leave the range of 32): NS_PARTS partial sums per matrix, fixed order
+#define NS_PARTS 64
+template <int DT> __global__ __launch_bounds__(256) void ns_norm_kernel(NsArgs a, double* part) {
+    const NsMat& m = a.m[blockIdx.y];
+    const int rows = m.tall ? m.t : m.s, cols = m.tall ? m.s : m.t;
+    const long long total = (long long)rows * cols;
+    double s = 0.0;
+    for (long long i = blockIdx.x * 256LL + threadIdx.x; i < total; i += NS_PARTS * 256LL) {
+        const long long r = i / cols;
+        const double v = ns_load<DT>(m.g, r * m.ldg + (i - r * cols));
+        s += v * v;
+    }
+    __shared__ double red[256];
+    red[threadIdx.x] = s;
+    __syncthreads();
+    for (int o = 128; o > 0; o >>= 1) {
+        if ((int)threadIdx.x < o) red[threadIdx.x] += red[threadIdx.x + o];
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) part[blockIdx.y * NS_PARTS + blockIdx.x] = red[0];
+}
+
+__device__ __forceinline__ void ns_put8(char* hi, const float* v) {          // eight scaled values -> their hi and lo halves
+    unsigned h[4], l[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) ga_split_pair_f16(v[2 * j], v[2 * j + 1], h[j], l[j]);
+    *(u32x4*)hi = u32x4{h[0], h[1], h[2], h[3]};
+    *(u32x4*)(hi + 64) = u32x4{l[0], l[1], l[2], l[3]};
+}
+__device__ __forceinline__ void ns_get8(const char* hi, float* v) {
+    const f16x8 h = *(const f16x8*)hi, l = *(const f16x8*)(hi + 64);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = (float)h[j] + (float)l[j];
+}
+
+// G / (|G|_F + eps) in both orientations, 64 x 64 values per workgroup turned through LDS
+template <int DT> __global__ __launch_bounds__(256) void ns_split_kernel(NsArgs a) {
+    __shared__ float tile[64][65];
+    __shared__ float scale_s;
+    const int mi = ns_find(a, blockIdx.x);
+    const NsMat& m = a.m[mi];
+    const int rows = m.tall ? m.t : m.s, cols = m.tall ? m.s : m.t;
+    const int ct = (cols + 63) / 64, id = blockIdx.x - a.first[mi], r0 = id / ct * 64, c0 = id % ct * 64;
+    if (threadIdx.x == 0) {
+        double s = 0.0;
+        for (int i = 0; i < NS_PARTS; ++i) s += a.part[mi * NS_PARTS + i];
+        scale_s = (float)((double)NS_SCALE / (sqrt(s) + (double)a.eps));
+    }
+    for (int i = threadIdx.x; i < 64 * 64; i += 256) {
+        const int r = r0 + (i >> 6), c = c0 + (i & 63);
+        tile[i >> 6][i & 63] = r < rows && c < cols ? ns_load<DT>(m.g, r * m.ldg + c) : 0.0f;
+    }
+    __syncthreads();
+    const float scale = scale_s;
+    char* direct = m.tall ? m.XT0 : m.X;      // [rows][cols]
+    char* turned = m.tall ? m.X : m.XT0;      // [cols][rows]
+#pragma unroll
+    for (int i = threadIdx.x; i < 512; i += 256) {
+        const int r = i >> 3, c = (i & 7) * 8;
+        float v[8];
+        if (r0 + r < rows && c0 + c < ns_r32(cols)) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = tile[r][c + j] * scale;
+            ns_put8(direct + (r0 + r) * ns_ld(cols) + ns_at(c0 + c), v);
+        }
+        if (c0 + r < cols && r0 + c < ns_r32(rows)) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = tile[c + j][r] * scale;
+            ns_put8(turned + (c0 + r) * ns_ld(rows) + ns_at(r0 + c), v);
+        }
+    }
+}
+
+template <int N> __device__ __forceinline__ void ns_wait() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+
+// One product tile.  S stages of LDS, S - 1 steps of fetches in flight.
+template <class C, int S, int KIND, int DT>
+__global__ __launch_bounds__(C::WAVES * 64) void ns_kernel(NsArgs a) {
+    constexpr int MT = C::MT, NT = C::NT;
+    __shared__ __attribute__((aligned(128))) char smem[S * C::STAGE];
+    static_assert(C::WAVES * 32 * 36 * 4 <= S * C::STAGE, "room for the turned tiles");
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave / C::WN, wn = wave % C::WN;
+    int blk;
+    {   // workgroup b runs on XCD b % 8: every XCD takes one contiguous run of tiles
+        const int nt = gridDim.x, q = nt >> 3, r = nt & 7, x = blockIdx.x & 7, i = blockIdx.x >> 3;
+        blk = x * q + (x < r ? x : r) + i;
+    }
+    const int mi = ns_find(a, blk);
+    const NsMat& mat = a.m[mi];
+    const int s = mat.s, t = mat.t, id = blk - a.first[mi];
+    const int M = s, N = KIND == NS_STEP ? t : s, K = KIND == NS_GRAM ? t : s;
+    int tm, tn;
+    if (KIND == NS_STEP) {
+        const int ntm = (M + C::BM - 1) / C::BM, ntn = (N + C::BN - 1) / C::BN;
+        const int width = 4 * ntn, g = id / width, f = 4 * g, sz = ntm - f < 4 ? ntm - f : 4;
+        tm = f + (id % width) % sz;
+        tn = (id % width) / sz;
+    } else {                                                          // row by row of the lower triangle
+        static_assert(KIND == NS_STEP || C::BM == C::BN, "square tiles on the diagonal");
+        tm = (int)((__builtin_sqrtf(8.0f * id + 1.0f) - 1.0f) * 0.5f);
+        while ((tm + 1) * (tm + 2) / 2 <= id) ++tm;
+        while (tm * (tm + 1) / 2 > id) --tm;
+        tn = id - tm * (tm + 1) / 2;
+    }
+    const int m0 = tm * C::BM, n0 = tn * C::BN;
+    const char* XT = a.flip ? mat.XT1 : mat.XT0;
+    const char* qp = KIND == NS_GRAM ? mat.X : KIND == NS_POLY ? mat.A : mat.B;
+    const char* pp = KIND == NS_GRAM ? mat.X : KIND == NS_POLY ? mat.A : XT;
+    const long long ldk = ns_ld(K);
+    MmLoad<MM_KC, C::BM, C::WAVES> lq;
+    MmLoad<MM_KC, C::BN, C::WAVES> lp;
+    lq.init(wave, lane, ldk, m0, M);
+    lp.init(wave, lane, ldk, n0, N);
+    qp += m0 * ldk;
+    pp += n0 * ldk;
+    const int T = ns_r32(K) / 32;
+    const unsigned smem0 = mm_lds_addr(smem);
+    auto issue = [&](int step, int buf) {
+        const unsigned lds = smem0 + buf * C::STAGE + wave * 1024;
+#pragma unroll
+        for (int i = 0; i < lq.NI; ++i) mm_dma_s(lq.off[i], qp + step * 128LL, lds + i * C::WAVES * 1024);
+#pragma unroll
+        for (int i = 0; i < lp.NI; ++i) mm_dma_s(lp.off[i], pp + step * 128LL, lds + C::QB + i * C::WAVES * 1024);
+    };
+    f32x16 acc[MT][NT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+    MmFrag<MM_KC, C::BM> fr;
+    fr.init(lane);
+
+    constexpr int PER = MmLoad<MM_KC, C::BM, C::WAVES>::NI + MmLoad<MM_KC, C::BN, C::WAVES>::NI;
+#pragma unroll
+    for (int i = 0; i < S - 1; ++i)
+        if (i < T) issue(i, i);
+    int buf = 0;
+    for (int step = 0; step < T; ++step) {
+        if (step + S - 2 < T) ns_wait<(S - 2) * PER>();               // S - 2 younger steps may still be on their way
+        else ns_wait<0>();
+        ga_lds_barrier();
+        if (step + S - 1 < T) issue(step + S - 1, buf == 0 ? S - 1 : buf - 1);
+        mm_lds* sm = (mm_lds*)smem + buf * C::STAGE;
+        buf = buf == S - 1 ? 0 : buf + 1;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            s16x8 ph[NT], pl[NT], qh[MT], ql[MT];
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                ph[j] = fr.get(sm, C::QB + fr.tile(wn * C::TN + 32 * j), k);
+                pl[j] = fr.get(sm, C::QB + fr.tile(wn * C::TN + 32 * j), 2 + k);
+            }
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                qh[i] = fr.get(sm, fr.tile(wm * C::TM + 32 * i), k);
+                ql[i] = fr.get(sm, fr.tile(wm * C::TM + 32 * i), 2 + k);
+            }
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) acc[i][j] = mm_mfma<false>(pl[j], qh[i], acc[i][j]);
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) acc[i][j] = mm_mfma<false>(ph[j], ql[i], acc[i][j]);
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) acc[i][j] = mm_mfma<false>(ph[j], qh[i], acc[i][j]);
+        }
+    }
+    ga_lds_barrier();
+
+    // Epilogue, one 32 x 32 tile of a wave at a time: [m][n] with 8 consecutive n per lane, then [n][m] with 8 consecutive m.
+    float* st = (float*)smem + wave * (32 * 36);
+    char* XTn = a.flip ? mat.XT0 : mat.XT1;
+    char* dst = KIND == NS_GRAM ? mat.A : KIND == NS_POLY ? mat.B : mat.X;
+    const char* old = KIND == NS_POLY ? mat.A : mat.X;
+    const long long ldn = ns_ld(N), ldm = ns_ld(M);
+    const bool user = KIND == NS_STEP && a.last;
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                *(f32x4*)(st + (lane & 31) * 36 + 8 * r + 4 * (lane >> 5)) =
+                    f32x4{acc[i][j][4 * r], acc[i][j][4 * r + 1], acc[i][j][4 * r + 2], acc[i][j][4 * r + 3]};
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            const int mb = m0 + wm * C::TM + 32 * i, nb = n0 + wn * C::TN + 32 * j;
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+                const int row = p * 16 + (lane >> 2), c = (lane & 3) * 8, m = mb + row, n = nb + c;
+                float v[8];
+                mm_ldf8(st + row * 36 + c, v);
+                if (m < M && n < ns_r32(N)) {
+                    if (KIND == NS_GRAM) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[e] *= 1.0f / NS_SCALE;
+                    } else {
+                        float x[8];
+                        ns_get8(old + m * ldn + ns_at(n), x);
+                        const float ca = KIND == NS_POLY ? a.b : a.a, cc = KIND == NS_POLY ? a.c / NS_SCALE : 1.0f / NS_SCALE;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[e] = ca * x[e] + cc * v[e];
+                    }
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] = n + e < N ? v[e] : 0.0f;
+                    if (!user) ns_put8(dst + m * ldn + ns_at(n), v);
+                    else if (!mat.tall) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            if (n + e < N) ns_store<DT>(mat.o, m * mat.ldo + n + e, v[e] * (1.0f / NS_SCALE));
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] = 0.0f;          // rows beyond the last are columns of zeros of the transpose
+                }
+                mm_stf8(st + row * 36 + c, v);
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            if (KIND == NS_STEP ? (!user || mat.tall) : tm != tn) {
+                char* tr = KIND == NS_STEP ? XTn : dst;
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    const int mc = p * 16 + (lane >> 5) * 8, n = nb + (lane & 31), m = mb + mc;
+                    float v[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] = st[(mc + e) * 36 + (lane & 31)];
+                    if (n < N && m < ns_r32(M)) {
+                        if (!user) ns_put8(tr + n * ldm + ns_at(m), v);
+                        else {
+#pragma unroll
+                            for (int e = 0; e < 8; ++e)
+                                if (m + e < M) ns_store<DT>(mat.o, n * mat.ldo + m + e, v[e] * (1.0f / NS_SCALE));
+                        }
+                    }
+                }
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        }
+}
+
+namespace {
+
+typedef MmGeom<64, 64, 4, 2> NsT;
+typedef MmGeom<128, 128, 4, 2> NsS;
+typedef MmGeom<192, 192, 4, 2> NsM;
+
+size_t al(size_t n) { return (n + 255) & ~(size_t)255; }
+
+// one matrix's planes; base may be null (only the size is wanted)
+size_t ns_planes(NsMat* m, char* base, int s, int t) {
+    const size_t x = al((size_t)s * ns_ld(t)), xt = al((size_t)t * ns_ld(s)), g = al((size_t)s * ns_ld(s));
+    if (m) { m->X = base; m->XT0 = base + x; m->XT1 = m->XT0 + xt; m->A = m->XT1 + xt; m->B = m->A + g; }
+    return x + 2 * xt + 2 * g;
+}
+
+long long tri(long long n) { return n * (n + 1) / 2; }
+
+// tiles of all matrices of the group for one product
+template <class C> int ns_tiles(NsArgs& a, int kind) {
+    long long at = 0;
+    for (int i = 0; i < a.count; ++i) {
+        a.first[i] = (int)at;
+        const long long r = (a.m[i].s + C::BM - 1) / C::BM, c = (a.m[i].t + C::BN - 1) / C::BN;
+        at += kind == NS_STEP ? r * c : tri(r);
+    }
+    a.first[a.count] = (int)at;
+    return (int)at;
+}
+
+template <class C, int S, int KIND, int DT> int ns_go(NsArgs& a, hipStream_t st) {
+    const int tiles = ns_tiles<C>(a, KIND);
+    hipLaunchKernelGGL((ns_kernel<C, S, KIND, DT>), dim3(tiles), dim3(C::WAVES * 64), 0, st, a);
+    return hipGetLastError() == hipSuccess ? ACMIL_OK : ACMIL_ERR_LAUNCH;
+}
+
+template <int KIND, int DT> int ns_product(NsArgs& a, hipStream_t st) {
+    // the largest tile that still gives most CUs work: larger tiles read less of LDS and L2 per flop
+    if (ns_tiles<NsM>(a, KIND) >= 200) return ns_go<NsM, 3, KIND, DT>(a, st);
+    if (ns_tiles<NsS>(a, KIND) >= 200) return ns_go<NsS, 2, KIND, DT>(a, st);
+    return ns_go<NsT, 6, KIND, DT>(a, st);
+}
+
+template <int DT> int ns_run(int count, const acmil_ortho_mat* mats, int steps, const float* co, float eps, char* ws, hipStream_t st) {
+    for (int at = 0; at < count; at += NS_GROUP) {                   // groups reuse the workspace: stream order
+        NsArgs a = {};
+        a.count = count - at < NS_GROUP ? count - at : NS_GROUP;
+        a.eps = eps;
+        double* part = (double*)ws;
+        a.part = part;
+        char* p = ws + al((size_t)NS_GROUP * NS_PARTS * 8);
+        long long blocks = 0;
+        for (int i = 0; i < a.count; ++i) {
+            const acmil_ortho_mat& u = mats[at + i];
+            NsMat& m = a.m[i];
+            m.g = u.g; m.o = u.o; m.ldg = u.ldg; m.ldo = u.ldo;
+            m.tall = u.m > u.n;
+            m.s = m.tall ? u.n : u.m; m.t = m.tall ? u.m : u.n;
+            p += ns_planes(&m, p, m.s, m.t);
+            a.first[i] = (int)blocks;
+            blocks += (long long)((u.m + 63) / 64) * ((u.n + 63) / 64);
+        }
+        a.first[a.count] = (int)blocks;
+        hipLaunchKernelGGL((ns_norm_kernel<DT>), dim3(NS_PARTS, a.count), dim3(256), 0, st, a, part);
+        hipLaunchKernelGGL((ns_split_kernel<DT>), dim3((unsigned)blocks), dim3(256), 0, st, a);
+        if (hipGetLastError() != hipSuccess) return ACMIL_ERR_LAUNCH;
+        for (int k = 0; k < steps; ++k) {
+            a.a = co[3 * k]; a.b = co[3 * k + 1]; a.c = co[3 * k + 2];
+            a.flip = k & 1;
+            a.last = k == steps - 1;
+            int rc = ns_product<NS_GRAM, ACMIL_DTYPE_F32>(a, st);
+            if (rc == ACMIL_OK) rc = ns_product<NS_POLY, ACMIL_DTYPE_F32>(a, st);
+            if (rc == ACMIL_OK) rc = ns_product<NS_STEP, DT>(a, st);
+            if (rc != ACMIL_OK) return rc;
+        }
+    }
+    return ACMIL_OK;
+}
+
+const int NS_MAX_DIM = 1 << 16, NS_MAX_STEPS = 64;
+
+int ns_check(int count, const acmil_ortho_mat* mats, int dtype) {
+    if (!mats) return ACMIL_ERR_NULL;
+    if (count <= 0) return ACMIL_ERR_SHAPE;
+    if (dtype != ACMIL_DTYPE_F32 && dtype != ACMIL_DTYPE_F16 && dtype != ACMIL_DTYPE_BF16) return ACMIL_ERR_UNSUPPORTED;
+    for (int i = 0; i < count; ++i) {
+        if (mats[i].m <= 0 || mats[i].n <= 0 || mats[i].m > NS_MAX_DIM || mats[i].n > NS_MAX_DIM) return ACMIL_ERR_SHAPE;
+        if (mats[i].ldg < mats[i].n || mats[i].ldo < mats[i].n) return ACMIL_ERR_SHAPE;
+    }
+    return ACMIL_OK;
+}
+
+// Do the polynomials keep the singular values, which start in [0, 1], where the scaled f16 halves can hold X, A and B?
+bool ns_coeffs_ok(int steps, const float* co) {
+    double u = 1.0;
+    for (int k = 0; k < steps; ++k) {
+        const double a = co[3 * k], b = co[3 * k + 1], c = co[3 * k + 2];
+        if (!std::isfinite(a + b + c)) return false;
+        double up = 0.0, bp = 0.0;
+        for (int i = 0; i <= 2048; ++i) {
+            const double s = u * i / 2048.0, q = b * s * s + c * s * s * s * s;
+            up = fmax(up, fabs(a * s + q * s));
+            bp = fmax(bp, fabs(q));
+        }
+        if (!(up <= 3.9) || !(bp <= 15.5)) return false;
+        u = up;
+    }
+    return true;
+}
+
+}  // namespace
+
+extern "C" size_t acmil_orthogonalize_workspace_bytes(int count, const acmil_ortho_mat* mats, int dtype) {
+    if (ns_check(count, mats, dtype) != ACMIL_OK) return 0;
+    size_t most = 0;
+    for (int at = 0; at < count; at += NS_GROUP) {
+        size_t n = 0;
+        for (int i = at; i < count && i < at + NS_GROUP; ++i) {
+            const bool tall = mats[i].m > mats[i].n;
+            n += ns_planes(nullptr, nullptr, tall ? mats[i].n : mats[i].m, tall ? mats[i].m : mats[i].n);
+        }
+        if (n > most) most = n;
+    }
+    return al((size_t)NS_GROUP * NS_PARTS * 8) + most;
+}
+
+extern "C" int acmil_orthogonalize(int count, const acmil_ortho_mat* mats, int dtype, int steps, const float* coeffs, float eps, void* workspace,
+                                   size_t workspace_bytes, void* stream) {
+    const int rc = ns_check(count, mats, dtype);
+    if (rc != ACMIL_OK) return rc;
+    if (!coeffs || !workspace) return ACMIL_ERR_NULL;
+    for (int i = 0; i < count; ++i)
+        if (!mats[i].g || !mats[i].o) return ACMIL_ERR_NULL;
+    if (steps < 1 || steps > NS_MAX_STEPS || !(eps >= 0.0f) || !ns_coeffs_ok(steps, coeffs)) return ACMIL_ERR_SHAPE;
+    if (((size_t)workspace & 255) != 0 || workspace_bytes < acmil_orthogonalize_workspace_bytes(count, mats, dtype)) return ACMIL_ERR_SHAPE;
+    hipStream_t st = (hipStream_t)stream;
+    if (dtype == ACMIL_DTYPE_F32) return ns_run<ACMIL_DTYPE_F32>(count, mats, steps, coeffs, eps, (char*)workspace, st);
+    if (dtype == ACMIL_DTYPE_F16) return ns_run<ACMIL_DTYPE_F16>(count, mats, steps, coeffs, eps, (char*)workspace, st);
+    return ns_run<ACMIL_DTYPE_BF16>(count, mats, steps, coeffs, eps, (char*)workspace, st);
+}

@@ -1149,3 +1149,51 @@ def gated_ffn_bwd(dy: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w_up:
     F = a.F
     return (dx, None if dgu is None else dgu[:F], None if dgu is None else dgu[f8:f8 + F], dd,
             None if bgu is None else bgu[:F], None if bgu is None else bgu[f8:f8 + F], bd)
+
+
+NS_COEFFS = (3.4445, -4.7750, 2.0315)      # drives singular values from [0.002, 1] into [0.68, 1.14] in 5 steps
+
+
+def orthogonalize(g, steps: int = 5, coeffs: Sequence = NS_COEFFS, eps: float = 1e-7):
+    """acmil_orthogonalize: the Newton-Schulz approximation of the orthogonal factor of each matrix (U V^T of G = U S V^T): X = G / (|G|_F + eps),
+    then `steps` times X <- a X + (b A + c A A) X with A = X X^T, on the transpose where a matrix is tall.
+    g: [m, n], a stack [..., m, n], or a list of [m, n] of any shapes (one type and device): all matrices share the launches.  fp32, fp16 or bf16,
+    returned in the same type and structure; values are held to 22 bits inside whatever the type.  coeffs: one (a, b, c) or one per step."""
+    lib = _lib.load()
+    many = isinstance(g, (list, tuple))
+    ts = list(g) if many else [g]
+    if not ts:
+        return []
+    _need_cuda(*ts)
+    dev, dt = ts[0].device, ts[0].dtype
+    if dt not in _DT or any(t.dtype != dt or t.device != dev for t in ts):
+        raise RuntimeError("acmil_amd.orthogonalize: fp32, fp16 or bf16 matrices of one type and one device")
+    if any(t.dim() != 2 for t in ts) if many else g.dim() < 2:
+        raise RuntimeError("acmil_amd.orthogonalize: [m, n], a stack [..., m, n] or a list of [m, n] expected")
+    table = [float(c) for c in coeffs] * steps if not isinstance(coeffs[0], (list, tuple)) else [float(c) for s in coeffs for c in s]
+    if steps < 1 or len(table) != 3 * steps:
+        raise ValueError("acmil_amd.orthogonalize: coeffs must be (a, b, c) or one (a, b, c) for each of the steps")
+    outs = [torch.empty(t.shape, dtype=dt, device=dev) for t in ts]
+    mats, hold = [], []
+    for t, o in zip(ts, outs):
+        if t.numel() == 0:
+            continue
+        m, n = t.shape[-2:]
+        t = t.detach()
+        t = t.reshape(-1, m, n) if t.dim() != 3 else t
+        if (n > 1 and t.stride(2) != 1) or (m > 1 and t.stride(1) < n):
+            t = t.contiguous()
+        hold.append(t)
+        size = t.element_size()
+        ld = t.stride(1) if m > 1 else n
+        for k in range(t.shape[0]):
+            mats.append(_lib.OrthoMat(t.data_ptr() + k * t.stride(0) * size, ld, o.data_ptr() + k * m * n * size, n, m, n))
+    if mats:
+        with torch.cuda.device(dev):
+            arr, co = (_lib.OrthoMat * len(mats))(*mats), (ctypes.c_float * len(table))(*table)
+            need = lib.acmil_orthogonalize_workspace_bytes(len(mats), arr, _DT[dt])
+            if need == 0:
+                raise RuntimeError("acmil_amd.orthogonalize: matrices of at most 65536 rows and columns")
+            ws = torch.empty(need, dtype=torch.uint8, device=dev)
+            _lib.check(lib.acmil_orthogonalize(len(mats), arr, _DT[dt], steps, co, float(eps), ws.data_ptr(), need, _stream()), "acmil_orthogonalize")
+    return outs if many else outs[0]

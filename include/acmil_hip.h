@@ -656,6 +656,26 @@ int acmil_gated_ffn(const acmil_ffn_args* args, void* workspace, size_t workspac
 size_t acmil_gated_ffn_bwd_workspace_bytes(const acmil_ffn_args* args);
 int acmil_gated_ffn_bwd(const acmil_ffn_args* args, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Orthogonalisation of weight updates by Newton-Schulz products (csrc/ortho.hip), for an optimizer that steps along the orthogonal
+ * factor of the momentum instead of the momentum itself (the reference's only optimizer is AdamW,
+ * Step3_WSI_classification_ACMIL.py:139; acmil_amd.optim.FlatMuon uses this one):
+ *   X = G / (|G|_F + eps);  for each (a, b, c):  A = X X^T, X <- a X + (b A + c A A) X   (on G^T where m > n);  o = X
+ * count matrices of one dtype (F32 / F16 / BF16) share the launches.  mats: HOST array; g [m,n] and o [m,n] row-major with leading
+ * dimensions ldg, ldo >= n (elements); o may be g.  1 <= m, n <= 65536.  coeffs: HOST array [steps][3], 1 <= steps <= 64; refused
+ * (ACMIL_ERR_SHAPE) unless the polynomials keep singular values that start in [0, 1] below 3.9 and |b s^2 + c s^4| below 15.5.
+ * Values are held as f16 pairs (22 bits) and products accumulate in fp32, whatever the type of g; the norm is formed in 64 bits.
+ * A zero matrix gives zeros; infinities or NaN in g give NaN.  Reproducible bit for bit.
+ * workspace: acmil_orthogonalize_workspace_bytes(...) (0 = refused), 256-byte aligned, contents arbitrary.
+ * ------------------------------------------------------------------------------------------- */
+typedef struct acmil_ortho_mat {
+    const void* g; long long ldg; void* o; long long ldo; int m, n;
+} acmil_ortho_mat;
+
+size_t acmil_orthogonalize_workspace_bytes(int count, const acmil_ortho_mat* mats, int dtype);
+int acmil_orthogonalize(int count, const acmil_ortho_mat* mats, int dtype, int steps, const float* coeffs, float eps, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

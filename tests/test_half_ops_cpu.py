@@ -87,3 +87,20 @@ def test_reference_gradients_are_those_of_differences(act):
     ref = R.ffn_ref(x, w, w * 0.5, w.t().contiguous(), None, None, None, act, None, x)
     for k, t in zip(("dx", "dwg", "dwu", "dwd"), grads):
         assert (ref[k].v - t).abs().max() < 1e-9 * (1 + t.abs().max()), k
+
+
+def test_orthogonalize_entry_refuses():
+    lib = _lib.load()
+    co = (ctypes.c_float * 15)(*([3.4445, -4.7750, 2.0315] * 5))
+
+    def call(m=8, n=16, ldg=16, ldo=16, dtype=0, steps=5, eps=1e-7, g=4096, o=4096, ws=4096, size=1 << 30, count=1, co=co):
+        mats = (_lib.OrthoMat * 1)(_lib.OrthoMat(g, ldg, o, ldo, m, n))
+        return lib.acmil_orthogonalize(count, mats, dtype, steps, co, eps, ws, size, None)
+
+    for kw, code in ((dict(m=0), -1), (dict(n=65537, ldg=1 << 17, ldo=1 << 17), -1), (dict(ldg=15), -1), (dict(ldo=15), -1), (dict(dtype=5), -2), (dict(steps=0), -1),
+                     (dict(steps=65), -1), (dict(eps=-1.0), -1), (dict(eps=float("nan")), -1), (dict(g=None), -3), (dict(o=None), -3), (dict(ws=None), -3),
+                     (dict(ws=4100), -1), (dict(size=100), -1), (dict(count=0), -1), (dict(co=None), -3),
+                     (dict(co=(ctypes.c_float * 15)(*([6.0, 0.0, 0.0] * 5))), -1), (dict(co=(ctypes.c_float * 15)(*([float("nan")] * 15))), -1)):
+        assert call(**kw) == code, kw
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        ops.orthogonalize(torch.zeros(4, 4))
