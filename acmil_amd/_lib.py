@@ -132,6 +132,8 @@ SIGNATURES = {
     "acmil_gated_ffn_bwd_workspace_bytes": (_sz, [_vp]),
     "acmil_gated_ffn_bwd": (_i, [_vp, _vp, _sz, _vp]),
     "acmil_orthogonalize_workspace_bytes": (_sz, [_i, _vp, _i]),
+    "acmil_muon_momentum": (_i, [_i, _vp, _vp, _vp, _vp, C.c_float, _i, _vp, _vp, _vp]),
+    "acmil_muon_apply": (_i, [_i, _vp, _vp, _vp, C.c_float, C.c_float, _vp, _vp]),
     "acmil_orthogonalize": (_i, [_i, _vp, _i, _i, C.POINTER(C.c_float), C.c_float, _vp, _sz, _vp]),
 }
 
@@ -165,6 +167,11 @@ class FfnArgs(C.Structure):
 class OrthoMat(C.Structure):
     """struct acmil_ortho_mat (include/acmil_hip.h)"""
     _fields_ = [("g", _vp), ("ldg", _ll), ("o", _vp), ("ldo", _ll), ("m", _i), ("n", _i)]
+
+
+class MuonSeg(C.Structure):
+    """struct acmil_muon_seg (include/acmil_hip.h)"""
+    _fields_ = [("offset", _ll), ("numel", _ll), ("scale", C.c_float)]
 
 
 _lib = None

@@ -1154,11 +1154,12 @@ def gated_ffn_bwd(dy: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w_up:
 NS_COEFFS = (3.4445, -4.7750, 2.0315)      # drives singular values from [0.002, 1] into [0.68, 1.14] in 5 steps
 
 
-def orthogonalize(g, steps: int = 5, coeffs: Sequence = NS_COEFFS, eps: float = 1e-7):
+def orthogonalize(g, steps: int = 5, coeffs: Sequence = NS_COEFFS, eps: float = 1e-7, out=None):
     """acmil_orthogonalize: the Newton-Schulz approximation of the orthogonal factor of each matrix (U V^T of G = U S V^T): X = G / (|G|_F + eps),
     then `steps` times X <- a X + (b A + c A A) X with A = X X^T, on the transpose where a matrix is tall.
     g: [m, n], a stack [..., m, n], or a list of [m, n] of any shapes (one type and device): all matrices share the launches.  fp32, fp16 or bf16,
-    returned in the same type and structure; values are held to 22 bits inside whatever the type.  coeffs: one (a, b, c) or one per step."""
+    returned in the same type and structure; values are held to 22 bits inside whatever the type.  coeffs: one (a, b, c) or one per step.
+    out: contiguous tensor(s) of g's structure, type and shapes to write to; g itself will do."""
     lib = _lib.load()
     many = isinstance(g, (list, tuple))
     ts = list(g) if many else [g]
@@ -1173,7 +1174,10 @@ def orthogonalize(g, steps: int = 5, coeffs: Sequence = NS_COEFFS, eps: float = 
     table = [float(c) for c in coeffs] * steps if not isinstance(coeffs[0], (list, tuple)) else [float(c) for s in coeffs for c in s]
     if steps < 1 or len(table) != 3 * steps:
         raise ValueError("acmil_amd.orthogonalize: coeffs must be (a, b, c) or one (a, b, c) for each of the steps")
-    outs = [torch.empty(t.shape, dtype=dt, device=dev) for t in ts]
+    outs = [torch.empty(t.shape, dtype=dt, device=dev) for t in ts] if out is None else list(out) if many else [out]
+    if out is not None and (len(outs) != len(ts) or any(o.shape != t.shape or o.dtype != dt or o.device != dev or not o.is_contiguous()
+                                                       for o, t in zip(outs, ts))):
+        raise RuntimeError("acmil_amd.orthogonalize: out must be contiguous tensors of g's structure, type and shapes")
     mats, hold = [], []
     for t, o in zip(ts, outs):
         if t.numel() == 0:

@@ -15,10 +15,12 @@ from typing import Callable, Iterable, List, Optional
 
 import torch
 
-from . import _lib
+from . import _lib, ops
 
 
 class FlatAdamW:
+    _muon_indices: Optional[List[int]] = None      # FlatMuon: which parameters take the orthogonalised step
+
     def __init__(self, params: Iterable[torch.nn.Parameter], lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 1e-2, grad_buffer: Optional[torch.Tensor] = None, on_step: Optional[Callable[[], None]] = None,
                  peer=None):
@@ -276,6 +278,8 @@ class FlatAdamW:
 
     def load_state_dict(self, sd):
         """Accepts torch.optim.AdamW's layout (also one written by the reference) or this class's earlier flat layout."""
+        if any("muon" in g for g in sd["param_groups"]) != (self._muon_indices is not None):
+            raise RuntimeError("acmil_amd.%s: this state was written by %s" % (type(self).__name__, "FlatMuon" if self._muon_indices is None else "another optimizer"))
         self._pending.clear()      # flags of steps taken before the load belong to the discarded state
         self.mutations += 1
         self.skipped_steps = 0
@@ -301,3 +305,99 @@ class FlatAdamW:
         self.exp_avg.copy_(sd["exp_avg"]); self.exp_avg_sq.copy_(sd["exp_avg_sq"])
         for g, s_ in zip(self.param_groups, sd["param_groups"]):
             g.update(s_)
+
+
+class FlatMuon(FlatAdamW):
+    """Orthogonalised momentum for the weight MATRICES, AdamW for everything else, over FlatAdamW's flat buffers:
+        buf = mu buf + g;  O = orthogonalize(nesterov ? g + mu buf : buf);  p = p (1 - lr wd) - lr 0.2 sqrt(max(m, n)) O
+    (0.2 sqrt(max(m, n)) gives an update the root mean square of AdamW's, so that learning rates and weight decays of AdamW carry over.)
+    A matrix is a 2-D parameter with both sides >= 32: projections and attention branches, not the score row of each branch or the class
+    heads; `muon` = the parameters themselves overrules that.  All matrices share the launches of one acmil_orthogonalize call.
+    The momentum lives in exp_avg.  A raised range flag skips the whole step on the device, as in FlatAdamW.  The update cannot run
+    inside the training step's own library call, and there is no direct peer reduction."""
+
+    def __init__(self, params: Iterable[torch.nn.Parameter], lr: float = 1e-3, momentum: float = 0.95, nesterov: bool = True, ns_steps: int = 5,
+                 betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, grad_buffer: Optional[torch.Tensor] = None,
+                 on_step: Optional[Callable[[], None]] = None, muon: Optional[Iterable[torch.nn.Parameter]] = None):
+        super().__init__(params, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, grad_buffer=grad_buffer, on_step=on_step)
+        if not 0.0 <= momentum < 1.0 or ns_steps < 1:
+            raise ValueError("acmil_amd.FlatMuon: 0 <= momentum < 1 and ns_steps >= 1")
+        chosen = None if muon is None else {id(p) for p in muon}
+        known = {id(p) for p in self.params}
+        if chosen is not None and not chosen <= known:
+            raise RuntimeError("acmil_amd.FlatMuon: muon holds tensors that are not among the trained parameters")
+        segs, self._runs, self._muon_indices, off, at, views = [], [], [], 0, 0, []
+        for i, p in enumerate(self.params):
+            n = p.numel()
+            if id(p) in chosen if chosen is not None else p.dim() == 2 and min(p.shape) >= 32:
+                if p.dim() != 2 or n == 0:
+                    raise RuntimeError("acmil_amd.FlatMuon: only matrices can be orthogonalised, got %s" % (tuple(p.shape),))
+                segs.append(_lib.MuonSeg(off, n, 0.2 * math.sqrt(max(p.shape))))
+                views.append((at, p.shape))
+                at += n
+                self._muon_indices.append(i)
+            elif self._runs and self._runs[-1][1] == off:
+                self._runs[-1][1] = off + n                       # neighbours go through one AdamW launch
+            else:
+                self._runs.append([off, off + n])
+            off += n
+        if not segs:
+            raise RuntimeError("acmil_amd.FlatMuon: no weight matrix among the parameters; use FlatAdamW")
+        self._segs = (_lib.MuonSeg * len(segs))(*segs)
+        self._update = torch.empty(at, dtype=torch.float32, device=self.flat.device)
+        self._update_views = [self._update[a:a + s.numel()].view(s) for a, s in views]
+        self._run_skips = torch.zeros(max(1, len(self._runs)), dtype=torch.int32, device=self.flat.device)      # one counter per AdamW launch
+        self.param_groups[0].update(momentum=momentum, nesterov=bool(nesterov), ns_steps=int(ns_steps))
+
+    def can_run_in_step(self) -> bool:
+        return False
+
+    @torch.no_grad()
+    def step(self, track_flag: bool = False) -> int:
+        g = self.param_groups[0]
+        track = track_flag and self.guard_flag is not None
+        if track and len(self._pending) >= 12:
+            raise RuntimeError("acmil_amd.FlatMuon: poll_skipped() must be called while steps are tracked")
+        self.step_count += 1
+        self._step_id += 1
+        self._launches += 1
+        slot = self._step_id % 16
+        lib, b1, b2 = _lib.load(), *g["betas"]
+        kept = [(o, self.flat[o:o + n].clone()) for o, n in self._frozen]
+        flag = None if self.guard_flag is None else self.guard_flag.data_ptr()
+        stream = torch.cuda.current_stream().cuda_stream
+        _lib.check(lib.acmil_muon_momentum(len(self._segs), self._segs, self.grad.data_ptr(), self.exp_avg.data_ptr(), self._update.data_ptr(),
+                                           float(g["momentum"]), int(g["nesterov"]), flag, self._host_flags.data_ptr() + 4 * slot if track else None,
+                                           stream), "acmil_muon_momentum")
+        ops.orthogonalize(self._update_views, steps=g["ns_steps"], out=self._update_views)
+        _lib.check(lib.acmil_muon_apply(len(self._segs), self._segs, self.flat.data_ptr(), self._update.data_ptr(), float(g["lr"]),
+                                        float(g["weight_decay"]), flag, stream), "acmil_muon_apply")
+        for i, (a, b) in enumerate(self._runs):
+            _lib.check(lib.acmil_adamw_step(self.flat.data_ptr() + 4 * a, self.grad.data_ptr() + 4 * a, self.exp_avg.data_ptr() + 4 * a,
+                                            self.exp_avg_sq.data_ptr() + 4 * a, b - a, float(g["lr"]), float(b1), float(b2), float(g["eps"]),
+                                            float(g["weight_decay"]), self._launches, flag, self._run_skips.data_ptr() + 4 * i, stream), "acmil_adamw_step")
+        for o, v in kept:
+            self.flat[o:o + v.numel()].copy_(v)
+        self.mutations += 1
+        if self.on_step is not None:
+            self.on_step()
+        if track:
+            ev = torch.cuda.Event()
+            ev.record()
+            self._pending.append((self._step_id, ev, slot))
+        return self._step_id
+
+    def state_dict(self):
+        """FlatAdamW's layout (a matrix's exp_avg is its momentum, its exp_avg_sq stays zero); the group also names the matrices."""
+        sd = super().state_dict()
+        g = self.param_groups[0]
+        sd["param_groups"][0].update(muon=list(self._muon_indices), momentum=g["momentum"], nesterov=g["nesterov"], ns_steps=g["ns_steps"])
+        return sd
+
+    def load_state_dict(self, sd):
+        group = sd["param_groups"][0]
+        if "muon" in group and list(group["muon"]) != self._muon_indices:
+            raise RuntimeError("acmil_amd.FlatMuon: the state's matrices are other parameters than this optimizer's")
+        super().load_state_dict(sd)
+        self._run_skips.zero_()
+        self.param_groups[0].update({k: group[k] for k in ("momentum", "nesterov", "ns_steps") if k in group})

@@ -516,6 +516,21 @@ def make_optimizer(model, conf, device, bucket: Optional["GradBucket"] = None, l
     """AdamW as in Step3_WSI_classification_ACMIL.py:139.  On the GPU: acmil_amd.optim.FlatAdamW (same update rule, parameters /
     gradients / moments in flat buffers, ONE launch per step; shares the DP gradient bucket); on CPU (gloo tests): torch's."""
     params = [p for p in model.parameters() if p.requires_grad]
+    if getattr(conf, "optimizer", "adamw") == "muon":
+        # --optimizer muon: orthogonalised momentum for the weight matrices, AdamW for the rest (optim.FlatMuon).  It reads gradients that
+        # are final: a data-parallel run reduces the bucket with torch.distributed, not inside the optimizer launch
+        if device.type != "cuda":
+            raise RuntimeError("acmil_amd.train: --optimizer muon needs the GPU (acmil_orthogonalize has no CPU form)")
+        from .optim import FlatMuon
+        if bucket is not None and bucket.peer is not None:
+            print("acmil_amd.train: --dp-reduce direct needs FlatAdamW; using torch.distributed all_reduce with FlatMuon")
+            bucket.peer.close()
+            bucket.peer = None
+        opt = FlatMuon(params, lr=lr, weight_decay=conf.wd, grad_buffer=None if bucket is None else bucket.flat,
+                       on_step=getattr(model, "invalidate_packed", None))
+        if getattr(conf, "arch", "") == "ga" and getattr(conf, "n_token", 2) == 1:
+            opt.set_frozen(list(model.classifier[0].parameters()))
+        return opt
     if device.type == "cuda" and not getattr(conf, "torch_optimizer", False):
         from .optim import FlatAdamW
         opt = FlatAdamW(params, lr=lr, weight_decay=conf.wd, grad_buffer=None if bucket is None else bucket.flat,
@@ -573,6 +588,8 @@ def get_arguments(argv=None):
                    help="slides per optimizer step and rank: > 1 trains on the MEAN gradient of that many slides per step (one batched "
                         "group step on the GPU; under data parallelism one all-reduce per group) -- the throughput mode; 1 = the "
                         "reference's B = 1 SGD (Step3_WSI_classification_ACMIL.py:189-221)")
+    p.add_argument("--optimizer", default="adamw", choices=["adamw", "muon"],
+                   help="adamw as the reference; muon: momentum orthogonalised by Newton-Schulz products for the weight matrices, AdamW for the rest")
     p.add_argument("--dp-reduce", dest="dp_reduce", default=os.environ.get("ACMIL_DP_REDUCE", "rccl"), choices=["rccl", "direct"],
                    help="data-parallel gradient reduction: torch.distributed all_reduce (RCCL), or the one-shot direct reduction fused "
                         "into the optimizer launch (peers' buckets read through IPC-mapped pointers; one node; falls back to rccl)")

@@ -676,6 +676,18 @@ size_t acmil_orthogonalize_workspace_bytes(int count, const acmil_ortho_mat* mat
 int acmil_orthogonalize(int count, const acmil_ortho_mat* mats, int dtype, int steps, const float* coeffs, float eps, void* workspace,
                         size_t workspace_bytes, void* stream);
 
+/* The element-wise passes around it in an optimizer step over flat fp32 buffers.  segs: HOST array of count matrices, [offset, offset +
+ * numel) in the flat buffers; `update` holds them packed, one behind the other in the order of segs.
+ *   acmil_muon_momentum: momentum = mu momentum + grads; update = nesterov ? grads + mu momentum : momentum
+ *   acmil_muon_apply:    params = params (1 - lr weight_decay) - lr scale update
+ * skip_flag / flag_report: as acmil_adamw_step_report -- a raised flag leaves momentum and params untouched. */
+typedef struct acmil_muon_seg { long long offset, numel; float scale; } acmil_muon_seg;
+
+int acmil_muon_momentum(int count, const acmil_muon_seg* segs, const float* grads, float* momentum, float* update, float mu, int nesterov,
+                        const float* skip_flag, float* flag_report, void* stream);
+int acmil_muon_apply(int count, const acmil_muon_seg* segs, float* params, const float* update, float lr, float weight_decay,
+                     const float* skip_flag, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -104,3 +104,19 @@ def test_orthogonalize_entry_refuses():
         assert call(**kw) == code, kw
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         ops.orthogonalize(torch.zeros(4, 4))
+
+
+def test_muon_entries_and_trainer_option_refuse():
+    from acmil_amd import train as T
+    lib = _lib.load()
+    seg = (_lib.MuonSeg * 2)(_lib.MuonSeg(0, 10, 1.0), _lib.MuonSeg(10, 0, 1.0))
+    assert lib.acmil_muon_momentum(2, seg, 4096, 4096, 4096, 0.9, 1, None, None, None) == -1          # an empty segment
+    assert lib.acmil_muon_momentum(1, seg, 4096, 4096, None, 0.9, 1, None, None, None) == -3
+    assert lib.acmil_muon_momentum(1, seg, 4096, 4096, 4096, 1.0, 1, None, None, None) == -1
+    assert lib.acmil_muon_momentum(0, seg, 4096, 4096, 4096, 0.9, 1, None, None, None) == -1
+    assert lib.acmil_muon_apply(1, None, 4096, 4096, 0.1, 0.0, None, None) == -3
+    assert lib.acmil_muon_apply(1, seg, None, 4096, 0.1, 0.0, None, None) == -3
+    with pytest.raises(RuntimeError, match="needs the GPU"):
+        T.make_optimizer(torch.nn.Linear(64, 64), T.Struct(wd=0.0, optimizer="muon"), torch.device("cpu"))
+    with pytest.raises(SystemExit):
+        T.get_arguments(["--optimizer", "sgd"])

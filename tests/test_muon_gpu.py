@@ -1,0 +1,145 @@
+"""optim.FlatMuon and `train --optimizer muon`: orthogonalised momentum for the matrices, AdamW for the rest."""
+import math
+
+import pytest
+import torch
+
+from acmil_amd import ops
+from acmil_amd.optim import FlatAdamW, FlatMuon
+from test_ortho_gpu import iterate
+
+pytestmark = pytest.mark.gpu
+SHAPES = [(64, 96), (96,), (5, 96), (40, 40), (32, 200), (7, 3, 3), (200, 33)]
+MATRICES = [0, 3, 4, 6]
+
+
+def parameters(seed=0):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.nn.Parameter((torch.randn(*s, generator=g) * 0.1).cuda()) for s in SHAPES]
+
+
+def set_grads(params, seed):
+    g = torch.Generator().manual_seed(100 + seed)
+    for p in params:
+        p.grad.copy_(torch.randn(*p.shape, generator=g) * 1e-2)
+
+
+@pytest.mark.parametrize("nesterov", [True, False])
+def test_steps_follow_the_formula(nesterov):
+    """Matrices against the formula in 64 bits: an update is off by at most lr scale times the orthogonalisation's own bound (test_ortho_gpu), the
+    momentum and the parameter by roundings of 2^-24 each (8 of them per step are allowed).  The rest is FlatAdamW bit for bit."""
+    params, twin = parameters(), parameters()
+    opt = FlatMuon(params, lr=1e-2, weight_decay=0.1, nesterov=nesterov)
+    ref = FlatAdamW(twin, lr=1e-2, weight_decay=0.1)
+    assert opt._muon_indices == MATRICES
+    want = {i: params[i].detach().double() for i in MATRICES}
+    buf = {i: torch.zeros_like(want[i]) for i in MATRICES}
+    slack = {i: 0.0 for i in MATRICES}
+    for step in range(4):
+        lr = 1e-2 / (1 + step)
+        opt.param_groups[0]["lr"] = ref.param_groups[0]["lr"] = lr
+        set_grads(params, step), set_grads(twin, step)
+        opt.step(), ref.step()
+        for i in MATRICES:
+            g = params[i].grad.double()
+            buf[i] = 0.95 * buf[i] + g
+            o, bound = iterate(g + 0.95 * buf[i] if nesterov else buf[i], torch.float64)
+            scale = 0.2 * math.sqrt(max(want[i].shape))
+            want[i] = want[i] * (1 - lr * 0.1) - lr * scale * o
+            slack[i] += lr * scale * (bound + 3.9 ** 5 * 2 ** -22) + 8 * 2 ** -24 * float(want[i].norm())
+            assert (params[i].double() - want[i]).norm() <= slack[i], (step, i)
+        for i, (p, q) in enumerate(zip(params, twin)):
+            if i not in MATRICES:
+                assert torch.equal(p, q), (step, i)
+
+
+def test_a_raised_flag_skips_the_step():
+    params = parameters()
+    opt = FlatMuon(params, lr=1e-2)
+    set_grads(params, 0)
+    opt.guard_flag.zero_()
+    opt.step(track_flag=True)
+    before, momentum = opt.flat.clone(), opt.exp_avg.clone()
+    opt.guard_flag.fill_(1.0)
+    opt.step(track_flag=True)
+    assert torch.equal(opt.flat, before) and torch.equal(opt.exp_avg, momentum)
+    assert opt.poll_skipped(0) == [2] and opt.skipped_steps == 1 and opt._run_skips.tolist() == [1] * len(opt._runs)
+    opt.guard_flag.zero_()
+    twin = parameters()
+    other = FlatMuon(twin, lr=1e-2)
+    for k in (0, 1):
+        set_grads(twin, k)
+        other.step()
+    set_grads(params, 1)
+    opt.step()
+    assert torch.equal(opt.flat, other.flat)                       # the skipped step left no trace, bias corrections included
+
+
+def test_state_and_choice_of_matrices():
+    params = parameters()
+    opt = FlatMuon(params, lr=1e-2, momentum=0.9, ns_steps=3, muon=[params[0], params[2]])
+    assert opt._muon_indices == [0, 2]
+    for k in range(2):
+        set_grads(params, k)
+        opt.step()
+    sd = opt.state_dict()
+    again = FlatMuon(parameters(), lr=1.0, muon=None)
+    with pytest.raises(RuntimeError, match="other parameters"):
+        again.load_state_dict(sd)
+    twin = [torch.nn.Parameter(p.detach().clone()) for p in params]
+    new = FlatMuon(twin, lr=1.0, muon=[twin[0], twin[2]])
+    new.load_state_dict(sd)
+    assert new.param_groups[0]["momentum"] == 0.9 and new.param_groups[0]["ns_steps"] == 3 and new.param_groups[0]["lr"] == 1e-2
+    set_grads(params, 5), set_grads(twin, 5)
+    opt.step(), new.step()
+    assert torch.equal(opt.flat, new.flat)
+    adam = FlatAdamW(parameters(), lr=1e-2)
+    with pytest.raises(RuntimeError, match="FlatMuon"):
+        adam.load_state_dict(sd)
+    with pytest.raises(RuntimeError, match="another optimizer"):
+        opt.load_state_dict(adam.state_dict())
+    for bad in (dict(muon=[params[1]]), dict(muon=[torch.nn.Parameter(torch.zeros(40, 40, device="cuda"))])):
+        with pytest.raises(RuntimeError):
+            FlatMuon(params, **bad)
+    with pytest.raises(RuntimeError, match="no weight matrix"):
+        FlatMuon([torch.nn.Parameter(torch.zeros(9, device="cuda"))])
+    with pytest.raises(ValueError):
+        FlatMuon(parameters(), momentum=1.0)
+
+
+def test_more_matrices_than_one_launch_holds():
+    g = torch.Generator().manual_seed(0)
+    params = [torch.nn.Parameter((torch.randn(32, 32 + k % 3, generator=g) * 0.1).cuda()) for k in range(70)]
+    opt = FlatMuon(params, lr=1e-2, weight_decay=0.0, nesterov=False)
+    start = [p.detach().clone() for p in params]
+    for k, p in enumerate(params):
+        p.grad.copy_(torch.randn(*p.shape, generator=g))
+    opt.step()
+    for k in (0, 23, 24, 63, 64, 69):
+        o = ops.orthogonalize(params[k].grad)
+        want = start[k] - 1e-2 * 0.2 * math.sqrt(max(params[k].shape)) * o
+        assert (params[k] - want).abs().max() <= 2 ** -22 * (start[k].abs().max() + 0.1)       # two roundings of values below 0.6
+
+
+@pytest.mark.parametrize("n_token, bags", [(5, 1), (1, 1), (5, 4)])
+def test_trainer_runs_with_muon(n_token, bags):
+    """train.train_one_epoch with the optimizer make_optimizer builds for --optimizer muon: runs, applies every step, moves every trained
+    parameter, and leaves the frozen branch head of an n_token = 1 model alone"""
+    from acmil_amd import train as T
+    args = T.get_arguments(["--optimizer", "muon", "--n_token", str(n_token)])
+    assert args.optimizer == "muon" and T.get_arguments([]).optimizer == "adamw"
+    dev = torch.device("cuda", 0)
+    conf = T.Struct(train_epoch=1, warmup_epoch=0, wd=1e-5, lr=1e-3, min_lr=0, n_class=3, n_token=n_token, n_masked_patch=10, mask_drop=0.6, arch="ga",
+                    precision="f16x3", seed=0, D_feat=512, D_inner=256, optimizer="muon", bags_per_step=bags)
+    T.set_seed(0)
+    model = T.build_model(conf).to(dev).train()
+    opt = T.make_optimizer(model, conf, dev, None, lr=conf.lr)
+    names = [n for n, p in model.named_parameters()]
+    assert [names[i] for i in opt._muon_indices] == ["dimreduction.fc1.weight", "attention.attention_V.0.weight", "attention.attention_U.0.weight"]
+    before = {n: p.detach().clone() for n, p in model.named_parameters()}
+    T.train_one_epoch(model, T.SyntheticBags(8, 700, 512, 3, seed=1), opt, dev, 0, conf, log_every=0)
+    opt.poll_skipped(0)
+    assert opt.step_count == 8 // bags and opt.skipped_steps == 0
+    for n, p in model.named_parameters():
+        assert torch.isfinite(p).all()
+        assert torch.equal(p, before[n]) == (n_token == 1 and n.startswith("classifier.0")), n
