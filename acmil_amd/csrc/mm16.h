@@ -33,6 +33,7 @@ struct MmArgs {
     MmEpi e;
 };
 
+// K steps of mm16_kernel.h
 static inline int mm_steps(const MmArgs& a) { return a.segs * ((((a.Kq > a.Kp) ? a.Kq : a.Kp) + 63) / 64); }
 int mm_launch_fwd(const MmArgs& a, bool bf, int epi, bool dual, bool large, hipStream_t st);     // P, Q with K contiguous
 int mm_launch_dgrad(const MmArgs& a, bool bf, int epi, bool large, hipStream_t st);              // P with K strided

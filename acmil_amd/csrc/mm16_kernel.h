@@ -1,12 +1,12 @@
-// mm16_kernel.h -- out[M, N] = sum_k Q(m, k) P(n, k) of fp16 / bf16 operands on v_mfma_f32_32x32x16, fp32 accumulation.
+// mm16_kernel.h -- out[M, N] = sum_k Q(m, k) P(n, k) of fp16 / bf16 operands on v_mfma_f32_16x16x32, fp32 accumulation.
 //
 // Every product of a linear layer and of a gated feed-forward block is this one with another choice of which dimension is
 // contiguous (MM_KC / MM_KS):   y = x W^T: P = W (KC), Q = x (KC);   dx = dz W: P = W (KS), Q = dz (KC);
 // dW = dz^T x: P = x (KS), Q = dz (KS).  DUAL multiplies the same Q by two P (gate and up projection) so that one wave holds both
 // factors of an output element in its accumulators and the product needs no second pass.
 //
-// Layout.  A K step is 64 wide.  Tiles travel global -> LDS by 16-byte LDS-DMA (no registers), two stages, one barrier a step: the
-// DMA of step t + 1 runs under the matrix instructions of step t.  The LDS image is linear in the DMA's lane order, so bank
+// Layout.  A K step is 64 wide.  Tiles travel global -> LDS by 16-byte LDS-DMA (no registers) through a ring of two stages, one barrier
+// a step.  The LDS image is linear in the DMA's lane order, so bank
 // conflicts are avoided by permuting which 16-byte chunk of its row each LANE FETCHES.  K-strided tiles lie in LDS as they lie in
 // memory ([k][row]) and are read by ds_read_b64_tr_b16, which hands every lane four consecutive k of its row: no transposed copy of
 // an operand is ever made.  P feeds the A side of the instruction: a lane then owns 4 consecutive COLUMNS of an output row.
@@ -15,6 +15,15 @@
 #pragma once
 #include "mm16.h"
 
+#include <utility>
+
+#define MM_INLINE __attribute__((always_inline))
+// f(0), f(1), ... f(N - 1) with constant arguments: register arrays must never be indexed by a variable
+template <class F, int... I> __device__ __forceinline__ void mm_for_(F f, std::integer_sequence<int, I...>) { (f(std::integral_constant<int, I>{}), ...); }
+template <int A, int B, class F> __device__ __forceinline__ void mm_for(F f) {
+    if constexpr (A < B) mm_for_([&](auto i) MM_INLINE { f(std::integral_constant<int, A + decltype(i)::value>{}); }, std::make_integer_sequence<int, B - A>{});
+}
+
 typedef __fp16 mm_h4 __attribute__((__vector_size__(4 * sizeof(__fp16))));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
@@ -22,13 +31,14 @@ typedef __attribute__((address_space(3))) char mm_lds;
 
 static __device__ __attribute__((aligned(16))) unsigned mm_zero[4];     // what a lane fetches in place of a chunk beyond K
 
-// tile geometry: WAVES waves, WN of them along the columns, each with MT x NT accumulator tiles of 32 x 32
+// Tile geometry: WAVES waves, WN of them along the columns, each with MT x NT accumulator tiles of 16 x 16.  One operand of one K step is
+// 128 bytes of every row (64 values, or 32 pairs of ortho.hip) and fills one slot of LDS.
 template <int BM_, int BN_, int WAVES_, int WN_> struct MmGeom {
     static constexpr int BM = BM_, BN = BN_, WAVES = WAVES_, WN = WN_;
-    static constexpr int TM = BM / (WAVES / WN), TN = BN / WN, MT = TM / 32, NT = TN / 32;
-    static constexpr int QB = BM * 128, PB = BN * 128, STAGE = QB + PB;
+    static constexpr int TM = BM / (WAVES / WN), TN = BN / WN, MT = TM / 16, NT = TN / 16;
+    static constexpr int QB = BM * 128, PB = BN * 128;
 };
-// LARGE: one 8-wave workgroup per CU (128 KB of LDS), else two 4-wave workgroups per CU
+// LARGE: one 8-wave workgroup per CU, else two 4-wave workgroups per CU; either way all 160 KB of LDS
 template <bool LARGE> struct MmCfg;
 template <> struct MmCfg<true> : MmGeom<256, 256, 8, 4> {};
 template <> struct MmCfg<false> : MmGeom<128, 128, 4, 2> {};
@@ -46,78 +56,74 @@ __device__ __forceinline__ void mm_dma_v(const char* src, unsigned lds) {
     asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 2\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
                  : "=&s"(keep) : "v"(src), "s"(lds) : "memory");
 }
-__device__ __forceinline__ void mm_wait_dma() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+template <int N> __device__ __forceinline__ void mm_wait_dma() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
 // chunk permutations: conflict-free for 8 lanes over 128 bytes and for 16 lanes over 256 bytes
-__device__ __forceinline__ int mm_swz_kc(int row) { return (row & 7) ^ ((row >> 3) & 1); }
-__device__ __forceinline__ int mm_swz_ks(int k) { return 2 * (k & 3) + 8 * (k & 1); }
+__device__ __forceinline__ int mm_swz_kc(int row) { return (row >> 1) & 7; }
+__device__ __forceinline__ int mm_swz_ks(int k) { return 2 * (k & 3) + 8 * ((k >> 3) & 1); }
 
-// One operand tile of R rows x 64 k: where a lane fetches from
+// One operand tile of R rows x one K step: where a lane fetches from
 template <int KIND, int R, int WAVES> struct MmLoad {
-    static constexpr int NI = R * 128 / (WAVES * 1024);             // DMA instructions per wave and stage
-    static constexpr int CPR = R / 8;                               // KS: 16-byte chunks per k row
+    static constexpr int NI = R * 128 / (WAVES * 1024);             // DMA instructions per wave and step
+    static constexpr int CPR = KIND == MM_KC ? 8 : R / 8;           // 16-byte chunks per row (KC: of one row, KS: of one k)
     unsigned off[NI];                                               // byte offset from the tile's base at k = 0
+    __device__ __forceinline__ static int row_of(int i, int wave, int lane) { return (i * WAVES + wave) * (64 / CPR) + lane / CPR; }
     __device__ __forceinline__ void init(int wave, int lane, long long ld, int row0, int rows) {
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
-            const int piece = i * WAVES + wave;
+            const int r = row_of(i, wave, lane);
             if (KIND == MM_KC) {
-                const int r = piece * 8 + (lane >> 3), c = (lane & 7) ^ mm_swz_kc(r);
-                const int rr = row0 + r < rows ? r : (rows - 1 - row0 > 0 ? rows - 1 - row0 : 0);   // rows beyond the last repeat it; never stored
+                const int c = (lane % CPR) ^ mm_swz_kc(r);
+                const int rr = row0 + r < rows ? r : rows - 1 - row0;                        // rows beyond the last repeat it; never stored
                 off[i] = (unsigned)(rr * ld) + c * 16;
             } else {
-                const int k = piece * (64 / CPR) + lane / CPR, c = (lane % CPR) ^ mm_swz_ks(k);
-                const int last = (rows - row0 + 7) / 8 - 1;
-                off[i] = (unsigned)(k * ld) + (c < last ? c : last) * 16;
+                const int c = (lane % CPR) ^ mm_swz_ks(r), last = (rows - row0 + 7) / 8 - 1;
+                off[i] = (unsigned)(r * ld) + (c < last ? c : last) * 16;
             }
         }
     }
     // k index (KC: of the chunk's first element) that instruction i of this lane fetches, relative to the step
     __device__ __forceinline__ static int k_of(int i, int wave, int lane) {
-        const int piece = i * WAVES + wave;
-        if (KIND == MM_KC) return 8 * ((lane & 7) ^ mm_swz_kc(piece * 8 + (lane >> 3)));
-        return piece * (64 / CPR) + lane / CPR;
+        const int r = row_of(i, wave, lane);
+        return KIND == MM_KC ? 8 * ((lane % CPR) ^ mm_swz_kc(r)) : r;
     }
 };
 
-template <int KIND, int R> struct MmFrag {                           // reading a 32-row x 16-k fragment out of LDS
+template <int KIND, int R> struct MmFrag {                           // reading 16-row x 32-k fragments of a wave out of LDS
     unsigned base;
-    int swz, lane;
-    __device__ __forceinline__ void init(int l) {
-        lane = l;
+    __device__ __forceinline__ void init(int l, int row0) {          // row0: the wave's first row, a multiple of 32
         if (KIND == MM_KC) {
-            const int r = l & 31;
-            base = r * 128 + ((((l >> 5)) ^ mm_swz_kc(r)) << 4);
-        } else {
-            const int k = 8 * (l >> 5) + ((l & 15) >> 2);
-            base = k * (R * 2) + (l & 1) * 8;
-            swz = mm_swz_ks(k);
+            const int r = l & 15;
+            base = (row0 + r) * 128 + (((l >> 4) ^ mm_swz_kc(r)) << 4);
+        } else {                                                     // the chunk permutation commutes with the (even) chunk a 16-row tile starts at
+            const int k = 8 * (l >> 4) + ((l & 15) >> 2);
+            base = k * (R * 2) + (((((l & 3) >> 1) ^ mm_swz_ks(k)) << 4) ^ (row0 * 2)) + (l & 1) * 8;
         }
     }
-    // KS: byte offset of the lane's chunk for the 32-row tile that starts at row
-    __device__ __forceinline__ unsigned tile(int row) const {
-        if (KIND == MM_KC) return row * 128;
-        return (((row >> 3) + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1)) ^ swz) << 4;
-    }
-    __device__ __forceinline__ s16x8 get(mm_lds* sm, unsigned tile_off, int s) const {
-        if (KIND == MM_KC) return *(const __attribute__((address_space(3))) s16x8*)(sm + (base ^ (s << 5)) + tile_off);
-        mm_lds* p = sm + base + tile_off + s * 16 * (R * 2);
+    // rows row0 + row .. + 15, the s-th 32 k of the step (pairs of ortho.hip: 0 the hi halves, 1 the lo halves)
+    __device__ __forceinline__ s16x8 get(mm_lds* sm, int row, int s) const {
+        if (KIND == MM_KC) return *(const __attribute__((address_space(3))) s16x8*)(sm + (base ^ (s << 6)) + row * 128);
+        mm_lds* p = sm + (base ^ (row * 2)) + s * 32 * (R * 2);
         const s16x4 lo = __builtin_bit_cast(s16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) mm_h4*)p));
         const s16x4 hi = __builtin_bit_cast(s16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) mm_h4*)(p + 4 * (R * 2))));
         return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     }
 };
 
-template <bool BF> __device__ __forceinline__ f32x16 mm_mfma(s16x8 a, s16x8 b, f32x16 c) {
-    if constexpr (BF) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-    else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+// The 16 x 16 x 32 form moves half the accumulator bytes per flop of the 32 x 32 x 16 one.  That is what counts: a loop of nothing
+// but these instructions runs into the power limit, at 2.02 PFLOP/s against 1.82 for the larger form (bf16, 256 CUs).
+template <bool BF> __device__ __forceinline__ f32x4 mm_mfma(s16x8 a, s16x8 b, f32x4 c) {
+    if constexpr (BF) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
 template <bool BF, int PK, int QK, int EPI, bool DUAL, bool LARGE>
 __global__ __launch_bounds__(MmCfg<LARGE>::WAVES * 64, 2) void mm16_kernel(MmArgs a) {
     using C = MmCfg<LARGE>;
     constexpr int MT = C::MT, NT = C::NT;
-    __shared__ __attribute__((aligned(128))) char smem[2 * C::STAGE];
+    constexpr int SLOT = C::QB, SLOTS = 5;                           // half a stage: one operand of one K step
+    static_assert(C::QB == C::PB, "either operand fits any slot");
+    __shared__ __attribute__((aligned(128))) char smem[SLOTS * SLOT];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / C::WN, wn = wave % C::WN;
 
@@ -142,91 +148,129 @@ __global__ __launch_bounds__(MmCfg<LARGE>::WAVES * 64, 2) void mm16_kernel(MmArg
         static_assert(!DUAL || PK == MM_KC, "two factors: K contiguous");
 #pragma unroll
         for (int i = 0; i < lp.NI; ++i) {
-            const int piece = i * C::WAVES + wave, r = piece * 8 + (lane >> 3), rf = r & (BNF - 1);
+            const int r = lp.row_of(i, wave, lane), rf = r & (BNF - 1);
             const int rr = n0 + rf < a.N ? rf : a.N - 1 - n0;
-            lp.off[i] = (unsigned)(rr * a.ldp) + ((lane & 7) ^ mm_swz_kc(r)) * 16;
+            lp.off[i] = (unsigned)(rr * a.ldp) + ((lane % lp.CPR) ^ mm_swz_kc(r)) * 16;
         }
     }
     const long long qbase = QK == MM_KC ? m0 * a.ldq : m0 * 2LL, pbase = PK == MM_KC ? n0 * a.ldp : n0 * 2LL;
-    const long long qstep = QK == MM_KC ? 128 : 64 * a.ldq, pstep = PK == MM_KC ? 128 : 64 * a.ldp;
-    const int kmax = a.Kq > a.Kp ? a.Kq : a.Kp, kmin = a.Kq < a.Kp ? a.Kq : a.Kp, tseg = (kmax + 63) >> 6, T = a.segs * tseg;
+    constexpr int BK = 64;                                           // K of a step
+    const long long qstep = QK == MM_KC ? 128 : BK * a.ldq, pstep = PK == MM_KC ? 128 : BK * a.ldp;
+    const int kmax = a.Kq > a.Kp ? a.Kq : a.Kp, kmin = a.Kq < a.Kp ? a.Kq : a.Kp, tseg = (kmax + BK - 1) / BK, T = a.segs * tseg;
     const int t0 = (int)((long long)T * blockIdx.y / a.splits), t1 = (int)((long long)T * (blockIdx.y + 1) / a.splits);
     const unsigned smem0 = mm_lds_addr(smem);
 
-    auto issue = [&](int t, int buf) {
+    // Fetching one operand of one step in NI pieces.  Fetches are never skipped, so that their count is a constant: behind the last step
+    // it is fetched again, unused.  TAIL (a K that is no multiple of 64): chunks beyond K come from the zero block.
+    constexpr int NI = decltype(lq)::NI;
+    struct Half { const char *from, *from2; unsigned lds; int k; };  // k: how much of K is left
+    auto half_of = [&](int t, int slot, bool rows) MM_INLINE {
+        t = t < t1 ? t : t1 - 1;
         const bool s1 = t >= tseg;                                   // segs <= 2
         const int tt = s1 ? t - tseg : t;
-        const char* qb = (s1 ? a.q1 : a.q0) + qbase + tt * qstep;
-        const char* pb = (s1 && !DUAL ? a.p1 : a.p0) + pbase + tt * pstep;
-        const char* pb2 = DUAL ? a.p1 + pbase + tt * pstep : pb;
-        const unsigned lds = smem0 + buf * C::STAGE + wave * 1024;
-        if (tt * 64 + 64 <= kmin) {
-#pragma unroll
-            for (int i = 0; i < lq.NI; ++i) mm_dma_s(lq.off[i], qb, lds + i * C::WAVES * 1024);
-#pragma unroll
-            for (int i = 0; i < lp.NI; ++i) mm_dma_s(lp.off[i], DUAL && i >= lp.NI / 2 ? pb2 : pb, lds + C::QB + i * C::WAVES * 1024);
-        } else {                                                     // the last step of a segment: chunks beyond K come from the zero block
-            const char* z = (const char*)mm_zero;
-#pragma unroll
-            for (int i = 0; i < lq.NI; ++i)
-                mm_dma_v(tt * 64 + lq.k_of(i, wave, lane) < a.Kq ? qb + lq.off[i] : z, lds + i * C::WAVES * 1024);
-#pragma unroll
-            for (int i = 0; i < lp.NI; ++i)
-                mm_dma_v(tt * 64 + lp.k_of(i, wave, lane) < a.Kp ? (DUAL && i >= lp.NI / 2 ? pb2 : pb) + lp.off[i] : z,
-                         lds + C::QB + i * C::WAVES * 1024);
-        }
+        Half h;
+        h.from = rows ? (s1 ? a.q1 : a.q0) + qbase + tt * qstep : (s1 && !DUAL ? a.p1 : a.p0) + pbase + tt * pstep;
+        h.from2 = DUAL && !rows ? a.p1 + pbase + tt * pstep : h.from;
+        h.lds = smem0 + slot * SLOT + wave * 1024;
+        h.k = (rows ? a.Kq : a.Kp) - tt * BK;
+        return h;
+    };
+    auto fetch_q = [&](const Half& x, auto piece, auto tail) MM_INLINE {
+        constexpr int i = decltype(piece)::value;
+        const unsigned lds = x.lds + i * C::WAVES * 1024;
+        if constexpr (!decltype(tail)::value) mm_dma_s(lq.off[i], x.from, lds);
+        else mm_dma_v(lq.k_of(i, wave, lane) < x.k ? x.from + lq.off[i] : (const char*)mm_zero, lds);
+    };
+    auto fetch_p = [&](const Half& x, auto piece, auto tail) MM_INLINE {
+        constexpr int i = decltype(piece)::value;
+        const unsigned lds = x.lds + i * C::WAVES * 1024;
+        const char* from = DUAL && i >= NI / 2 ? x.from2 : x.from;
+        if constexpr (!decltype(tail)::value) mm_dma_s(lp.off[i], from, lds);
+        else mm_dma_v(lp.k_of(i, wave, lane) < x.k ? from + lp.off[i] : (const char*)mm_zero, lds);
     };
 
-    f32x16 acc[MT][NT];
+    f32x4 acc[MT][NT];
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+        for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
     MmFrag<QK, C::BM> fq;
     MmFrag<PK, C::BN> fp;
-    fq.init(lane);
-    fp.init(lane);
-    unsigned qt[MT], pt[NT];
-#pragma unroll
-    for (int i = 0; i < MT; ++i) qt[i] = fq.tile(wm * C::TM + 32 * i);
-#pragma unroll
-    for (int j = 0; j < NT; ++j) pt[j] = C::QB + fp.tile(DUAL ? j * BNF + wn * 32 : wn * 64 + 32 * j);
+    fq.init(lane, wm * C::TM);
+    fp.init(lane, wn * (DUAL ? C::TN / 2 : C::TN));
 
-    if (t0 < t1) issue(t0, 0);
-    for (int t = t0; t < t1; ++t) {
-        const int buf = (t - t0) & 1;
-        mm_wait_dma();                                               // this wave's share of step t has landed ...
-        ga_lds_barrier();                                            // ... and everybody's; everybody is done reading step t - 1
-        if (t + 1 < t1) issue(t + 1, buf ^ 1);
-        mm_lds* sm = (mm_lds*)smem + buf * C::STAGE;
+    // The ring has five slots for Q_0 P_0 Q_1 P_1 Q_2 ...  A step is two pieces of 32 k.  A piece goes row tile by row tile: NT matrix
+    // instructions, then the row fragment just used is read again for the next piece (the column fragments, which every row tile needs,
+    // have two register sets).  Between the pieces of step t a wave has read all it needs of Q_t and P_t, and its share of Q_(t+1) and
+    // P_(t+1) has landed: behind the one barrier of the step the first fragments of step t + 1 are read.  Q_(t+2) is fetched during the
+    // first piece, into the slot that was free, and P_(t+2) during the second, into that of Q_t.  Fetches are spread over the step because
+    // one that finds the address unit busy holds its wave up, with its matrix instructions: sent out in one burst behind the barrier
+    // they cost 18 % more cycles.
+    s16x8 p[2][NT], q[MT];
+    auto read_p = [&](mm_lds* slot, auto ks, auto kf) MM_INLINE {
+        constexpr int sub = decltype(ks)::value, f = decltype(kf)::value;
+        p[sub][f] = fp.get(slot, DUAL ? (f / (NT / 2)) * BNF + (f % (NT / 2)) * 16 : 16 * f, sub);
+    };
+    auto read_q = [&](mm_lds* slot, auto ks, auto kf) MM_INLINE {
+        constexpr int sub = decltype(ks)::value, f = decltype(kf)::value;
+        q[f] = fq.get(slot, 16 * f, sub);
+    };
+    mm_lds* const ring = (mm_lds*)smem;
+    auto run = [&](auto tail) MM_INLINE {
+        // piece `sub` multiplies; fragments of the other piece are read from the given slots
+        auto piece = [&](auto ks, mm_lds* qslot, mm_lds* pslot, const Half& h) MM_INLINE {
+            constexpr int sub = decltype(ks)::value;
+            using Other = std::integral_constant<int, 1 - sub>;
+            mm_for<0, MT>([&](auto ki) MM_INLINE {
+                constexpr int i = decltype(ki)::value;
+                mm_for<i * NT / MT, (i + 1) * NT / MT>([&](auto f) MM_INLINE { read_p(pslot, Other{}, f); });
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            s16x8 p[NT], q[MT];
-#pragma unroll
-            for (int j = 0; j < NT; ++j) p[j] = fp.get(sm, pt[j], s);
-#pragma unroll
-            for (int i = 0; i < MT; ++i) q[i] = fq.get(sm, qt[i], s);
-#pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-                for (int j = 0; j < NT; ++j) acc[i][j] = mm_mfma<BF>(p[j], q[i], acc[i][j]);
+                for (int j = 0; j < NT; ++j) acc[i][j] = mm_mfma<BF>(p[sub][j], q[i], acc[i][j]);
+                __builtin_amdgcn_sched_barrier(0);                   // else the read goes first, into registers that are not there
+                read_q(qslot, Other{}, ki);
+                mm_for<i * NI / MT, (i + 1) * NI / MT>([&](auto d) MM_INLINE {
+                    if constexpr (sub == 0) fetch_q(h, d, tail);
+                    else fetch_p(h, d, tail);
+                });
+                __builtin_amdgcn_sched_barrier(0);
+            });
+        };
+        mm_for<0, 2>([&](auto i) MM_INLINE {
+            const Half hq = half_of(t0 + i, 2 * i, true), hp = half_of(t0 + i, 2 * i + 1, false);
+            mm_for<0, NI>([&](auto d) MM_INLINE { fetch_q(hq, d, tail); });
+            mm_for<0, NI>([&](auto d) MM_INLINE { fetch_p(hp, d, tail); });
+        });
+        mm_wait_dma<2 * NI>();
+        ga_lds_barrier();
+        int qs = 0, ps = 1, free = 4;                                // slots of Q_t, P_t and the one that Q_(t+2) goes to
+        mm_for<0, NT>([&](auto f) MM_INLINE { read_p(ring + SLOT, std::integral_constant<int, 0>{}, f); });
+        mm_for<0, MT>([&](auto f) MM_INLINE { read_q(ring, std::integral_constant<int, 0>{}, f); });
+        for (int t = t0; t < t1; ++t) {
+            const Half hq = half_of(t + 2, free, true), hp = half_of(t + 2, qs, false);
+            piece(std::integral_constant<int, 0>{}, ring + qs * SLOT, ring + ps * SLOT, hq);
+            mm_wait_dma<NI>();                                       // Q_(t+2) may still be on its way
+            ga_lds_barrier();
+            free = ps;
+            qs = qs >= SLOTS - 2 ? qs + 2 - SLOTS : qs + 2;
+            ps = ps >= SLOTS - 2 ? ps + 2 - SLOTS : ps + 2;
+            piece(std::integral_constant<int, 1>{}, ring + qs * SLOT, ring + ps * SLOT, hp);
         }
-    }
+    };
+    if (kmin == kmax && kmin % BK == 0) run(std::false_type{});
+    else run(std::true_type{});
+    mm_wait_dma<0>();
     ga_lds_barrier();                                                // the stages are free: the epilogue turns its tiles there
 
+    static_assert(C::TN == 64, "the epilogue turns 32 rows x 64 columns of a wave at a time (DUAL: 32 columns of both factors)");
     float* st = (float*)smem + wave * (32 * 68);
     const int mrow = m0 + wm * C::TM;
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
+    for (int i = 0; i < MT / 2; ++i) {
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
+        for (int ii = 0; ii < 2; ++ii)
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-                *(f32x4*)(st + (lane & 31) * 68 + 32 * j + 8 * r + 4 * (lane >> 5)) =
-                    f32x4{acc[i][j][4 * r], acc[i][j][4 * r + 1], acc[i][j][4 * r + 2], acc[i][j][4 * r + 3]};
+            for (int j = 0; j < NT; ++j) *(f32x4*)(st + (16 * ii + (lane & 15)) * 68 + 16 * j + 4 * (lane >> 4)) = acc[2 * i + ii][j];
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");           // a wave turns its own tile: its LDS operations are in order
         if constexpr (!DUAL) {
 #pragma unroll 1

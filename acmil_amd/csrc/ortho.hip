@@ -5,11 +5,11 @@
 // Arithmetic.  A single 16-bit product would not do: errors of the null directions are multiplied by a^steps (485 for 3.4445^5).  Every
 // value is held as a pair of f16 halves, hi + lo (22 bits and a common power-of-two scale, so that nothing is lost to the narrow
 // exponent: |X|, |A|, |B| are bounded by the polynomial, checked on the host), and a product is hi hi + hi lo + lo hi on
-// v_mfma_f32_32x32x16_f16 with fp32 accumulation -- as exact as an fp32 product at a multiple of its rate.
+// v_mfma_f32_16x16x32_f16 with fp32 accumulation -- as exact as an fp32 product at a multiple of its rate.
 //
 // Layout.  A row of K values lies as blocks of 32: 64 bytes of hi halves, then 64 bytes of lo halves.  A K step of 32 is then
-// exactly one 128-byte row piece, and tiles move and lie in LDS like those of mm16_kernel.h; of a fragment's four 16-wide pieces two
-// are hi and two lo.  K is padded to a multiple of 32 with zeros, so there is no tail.  All three products take both operands with K
+// exactly one 128-byte row piece, and tiles move and lie in LDS like those of mm16_kernel.h, the first of a fragment's two halves being hi, the
+// second lo.  K is padded to a multiple of 32 with zeros, so there is no tail.  All three products take both operands with K
 // contiguous: X is kept in both orientations (its transpose twice, read and written alternately).  A and B are symmetric: only tiles on
 // and below the diagonal are computed and each is written a second time, mirrored.
 // All matrices of a call go through the same launches: 2 + 3 steps of them, whatever the number of matrices (up to NS_GROUP at a time).
@@ -58,17 +58,21 @@ template <int DT> __device__ __forceinline__ void ns_store(void* p, long long i,
 }
 
 // sum of squares, in 64 bits (a gradient's squares leave the range of 32): NS_PARTS partial sums per matrix, fixed order
-#define NS_PARTS 64
+#define NS_PARTS 512
 template <int DT> __global__ __launch_bounds__(256) void ns_norm_kernel(NsArgs a, double* part) {
     const NsMat& m = a.m[blockIdx.y];
     const int rows = m.tall ? m.t : m.s, cols = m.tall ? m.s : m.t;
-    const long long total = (long long)rows * cols;
     double s = 0.0;
-    for (long long i = blockIdx.x * 256LL + threadIdx.x; i < total; i += NS_PARTS * 256LL) {
-        const long long r = i / cols;
-        const double v = ns_load<DT>(m.g, r * m.ldg + (i - r * cols));
-        s += v * v;
-    }
+    // a row per quarter of the workgroup: 64 lanes x 4 neighbouring values
+    const int lane = threadIdx.x & 63;
+    for (int r = blockIdx.x * 4 + (threadIdx.x >> 6); r < rows; r += NS_PARTS * 4)
+        for (int c = lane * 4; c < cols; c += 256) {
+            float v[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = c + j < cols ? ns_load<DT>(m.g, r * m.ldg + c + j) : 0.0f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s += (double)v[j] * (double)v[j];
+        }
     __shared__ double red[256];
     red[threadIdx.x] = s;
     __syncthreads();
@@ -100,10 +104,12 @@ template <int DT> __global__ __launch_bounds__(256) void ns_split_kernel(NsArgs 
     const NsMat& m = a.m[mi];
     const int rows = m.tall ? m.t : m.s, cols = m.tall ? m.s : m.t;
     const int ct = (cols + 63) / 64, id = blockIdx.x - a.first[mi], r0 = id / ct * 64, c0 = id % ct * 64;
-    if (threadIdx.x == 0) {
+    if (threadIdx.x < 64) {                                           // every workgroup adds the partial sums up for itself, in one order
         double s = 0.0;
-        for (int i = 0; i < NS_PARTS; ++i) s += a.part[mi * NS_PARTS + i];
-        scale_s = (float)((double)NS_SCALE / (sqrt(s) + (double)a.eps));
+        for (int i = threadIdx.x; i < NS_PARTS; i += 64) s += a.part[mi * NS_PARTS + i];
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+        if (threadIdx.x == 0) scale_s = (float)((double)NS_SCALE / (sqrt(s) + (double)a.eps));
     }
     for (int i = threadIdx.x; i < 64 * 64; i += 256) {
         const int r = r0 + (i >> 6), c = c0 + (i & 63);
@@ -130,14 +136,15 @@ template <int DT> __global__ __launch_bounds__(256) void ns_split_kernel(NsArgs 
     }
 }
 
-template <int N> __device__ __forceinline__ void ns_wait() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
-
-// One product tile.  S stages of LDS, S - 1 steps of fetches in flight.
-template <class C, int S, int KIND, int DT>
+// One product tile.  As in mm16_kernel.h, with 32 pairs a step and so one piece a step: the fragments of step t + 1 are read while those of
+// step t multiply, and behind the barrier in front of step t both slots of its stage are free.  D steps are in flight or being read.
+template <class C, int D, int KIND, int DT>
 __global__ __launch_bounds__(C::WAVES * 64) void ns_kernel(NsArgs a) {
     constexpr int MT = C::MT, NT = C::NT;
-    __shared__ __attribute__((aligned(128))) char smem[S * C::STAGE];
-    static_assert(C::WAVES * 32 * 36 * 4 <= S * C::STAGE, "room for the turned tiles");
+    constexpr int SLOT = C::QB, SLOTS = 2 * D + 1;
+    static_assert(C::QB == C::PB && D >= 2, "either operand fits any slot");
+    __shared__ __attribute__((aligned(128))) char smem[SLOTS * SLOT];
+    static_assert(C::WAVES * 32 * 36 * 4 <= SLOTS * SLOT, "room for the turned tiles");
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / C::WN, wn = wave % C::WN;
     int blk;
@@ -175,62 +182,75 @@ __global__ __launch_bounds__(C::WAVES * 64) void ns_kernel(NsArgs a) {
     pp += n0 * ldk;
     const int T = ns_r32(K) / 32;
     const unsigned smem0 = mm_lds_addr(smem);
-    auto issue = [&](int step, int buf) {
-        const unsigned lds = smem0 + buf * C::STAGE + wave * 1024;
-#pragma unroll
-        for (int i = 0; i < lq.NI; ++i) mm_dma_s(lq.off[i], qp + step * 128LL, lds + i * C::WAVES * 1024);
-#pragma unroll
-        for (int i = 0; i < lp.NI; ++i) mm_dma_s(lp.off[i], pp + step * 128LL, lds + C::QB + i * C::WAVES * 1024);
+    constexpr int NI = decltype(lq)::NI;
+    auto fetch = [&](bool rows, int step, int slot, auto piece) MM_INLINE {
+        constexpr int k = decltype(piece)::value;
+        const long long at = (step < T ? step : T - 1) * 128LL;      // behind the last step it is fetched again, unused
+        const unsigned lds = smem0 + slot * SLOT + (k * C::WAVES + wave) * 1024;
+        if (rows) mm_dma_s(lq.off[k], qp + at, lds);
+        else mm_dma_s(lp.off[k], pp + at, lds);
     };
-    f32x16 acc[MT][NT];
+    f32x4 acc[MT][NT];
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
-    MmFrag<MM_KC, C::BM> fr;
-    fr.init(lane);
-
-    constexpr int PER = MmLoad<MM_KC, C::BM, C::WAVES>::NI + MmLoad<MM_KC, C::BN, C::WAVES>::NI;
-#pragma unroll
-    for (int i = 0; i < S - 1; ++i)
-        if (i < T) issue(i, i);
-    int buf = 0;
-    for (int step = 0; step < T; ++step) {
-        if (step + S - 2 < T) ns_wait<(S - 2) * PER>();               // S - 2 younger steps may still be on their way
-        else ns_wait<0>();
+        for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    MmFrag<MM_KC, C::BM> fq;
+    MmFrag<MM_KC, C::BN> fp;
+    fq.init(lane, wm * C::TM);
+    fp.init(lane, wn * C::TN);
+    mm_lds* const ring = (mm_lds*)smem;
+    s16x8 ph[2][NT], pl[2][NT], qh[MT], ql[MT];
+    auto read_p = [&](mm_lds* slot, auto set, auto kf) MM_INLINE {
+        constexpr int x = decltype(set)::value, f = decltype(kf)::value;
+        ph[x][f] = fp.get(slot, 16 * f, 0);
+        pl[x][f] = fp.get(slot, 16 * f, 1);
+    };
+    auto read_q = [&](mm_lds* slot, auto kf) MM_INLINE {
+        constexpr int f = decltype(kf)::value;
+        qh[f] = fq.get(slot, 16 * f, 0);
+        ql[f] = fq.get(slot, 16 * f, 1);
+    };
+    mm_for<0, SLOTS>([&](auto h) MM_INLINE {
+        constexpr int k = decltype(h)::value;
+        mm_for<0, NI>([&](auto d) MM_INLINE { fetch(k % 2 == 0, k / 2, k, d); });
+    });
+    mm_wait_dma<NI * (2 * D - 1)>();
+    ga_lds_barrier();
+    int qs = 0, ps = 1;                                               // slots of Q_t and P_t
+    mm_for<0, NT>([&](auto f) MM_INLINE { read_p(ring + SLOT, std::integral_constant<int, 0>{}, f); });
+    mm_for<0, MT>([&](auto f) MM_INLINE { read_q(ring, f); });
+    auto step = [&](int t, auto set) MM_INLINE {
+        constexpr int x = decltype(set)::value;
+        mm_wait_dma<NI * (2 * D - 3)>();                              // stage t + 1 has landed, for everybody behind the barrier; stage t is read
         ga_lds_barrier();
-        if (step + S - 1 < T) issue(step + S - 1, buf == 0 ? S - 1 : buf - 1);
-        mm_lds* sm = (mm_lds*)smem + buf * C::STAGE;
-        buf = buf == S - 1 ? 0 : buf + 1;
+        const int nq = qs >= SLOTS - 2 ? qs + 2 - SLOTS : qs + 2, np = ps >= SLOTS - 2 ? ps + 2 - SLOTS : ps + 2;
+        mm_for<0, MT>([&](auto ki) MM_INLINE {
+            constexpr int i = decltype(ki)::value;
+            mm_for<i * NT / MT, (i + 1) * NT / MT>([&](auto f) MM_INLINE { read_p(ring + np * SLOT, std::integral_constant<int, 1 - x>{}, f); });
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            s16x8 ph[NT], pl[NT], qh[MT], ql[MT];
+            for (int j = 0; j < NT; ++j) acc[i][j] = mm_mfma<false>(pl[x][j], qh[i], acc[i][j]);          // the small products first
 #pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                ph[j] = fr.get(sm, C::QB + fr.tile(wn * C::TN + 32 * j), k);
-                pl[j] = fr.get(sm, C::QB + fr.tile(wn * C::TN + 32 * j), 2 + k);
-            }
+            for (int j = 0; j < NT; ++j) acc[i][j] = mm_mfma<false>(ph[x][j], ql[i], acc[i][j]);
 #pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                qh[i] = fr.get(sm, fr.tile(wm * C::TM + 32 * i), k);
-                ql[i] = fr.get(sm, fr.tile(wm * C::TM + 32 * i), 2 + k);
-            }
-#pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-                for (int j = 0; j < NT; ++j) acc[i][j] = mm_mfma<false>(pl[j], qh[i], acc[i][j]);
-#pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-                for (int j = 0; j < NT; ++j) acc[i][j] = mm_mfma<false>(ph[j], ql[i], acc[i][j]);
-#pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-                for (int j = 0; j < NT; ++j) acc[i][j] = mm_mfma<false>(ph[j], qh[i], acc[i][j]);
-        }
+            for (int j = 0; j < NT; ++j) acc[i][j] = mm_mfma<false>(ph[x][j], qh[i], acc[i][j]);
+            __builtin_amdgcn_sched_barrier(0);
+            read_q(ring + nq * SLOT, ki);
+            mm_for<i * 2 * NI / MT, (i + 1) * 2 * NI / MT>([&](auto d) MM_INLINE {
+                constexpr int k = decltype(d)::value;
+                if constexpr (k < NI) fetch(false, t + D, qs, d);
+                else fetch(true, t + D + 1, ps, std::integral_constant<int, k - NI>{});
+            });
+            __builtin_amdgcn_sched_barrier(0);
+        });
+        qs = nq;
+        ps = np;
+    };
+    for (int t = 0; t < T; t += 2) {
+        step(t, std::integral_constant<int, 0>{});
+        if (t + 1 < T) step(t + 1, std::integral_constant<int, 1>{});
     }
+    mm_wait_dma<0>();
     ga_lds_barrier();
 
     // Epilogue, one 32 x 32 tile of a wave at a time: [m][n] with 8 consecutive n per lane, then [n][m] with 8 consecutive m.
@@ -241,13 +261,13 @@ __global__ __launch_bounds__(C::WAVES * 64) void ns_kernel(NsArgs a) {
     const long long ldn = ns_ld(N), ldm = ns_ld(M);
     const bool user = KIND == NS_STEP && a.last;
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int i = 0; i < MT / 2; ++i)
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
+        for (int j = 0; j < NT / 2; ++j) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-                *(f32x4*)(st + (lane & 31) * 36 + 8 * r + 4 * (lane >> 5)) =
-                    f32x4{acc[i][j][4 * r], acc[i][j][4 * r + 1], acc[i][j][4 * r + 2], acc[i][j][4 * r + 3]};
+            for (int ii = 0; ii < 2; ++ii)
+#pragma unroll
+                for (int jj = 0; jj < 2; ++jj) *(f32x4*)(st + (16 * ii + (lane & 15)) * 36 + 16 * jj + 4 * (lane >> 4)) = acc[2 * i + ii][2 * j + jj];
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             const int mb = m0 + wm * C::TM + 32 * i, nb = n0 + wn * C::TN + 32 * j;
 #pragma unroll
@@ -332,17 +352,17 @@ template <class C> int ns_tiles(NsArgs& a, int kind) {
     return (int)at;
 }
 
-template <class C, int S, int KIND, int DT> int ns_go(NsArgs& a, hipStream_t st) {
+template <class C, int D, int KIND, int DT> int ns_go(NsArgs& a, hipStream_t st) {
     const int tiles = ns_tiles<C>(a, KIND);
-    hipLaunchKernelGGL((ns_kernel<C, S, KIND, DT>), dim3(tiles), dim3(C::WAVES * 64), 0, st, a);
+    hipLaunchKernelGGL((ns_kernel<C, D, KIND, DT>), dim3(tiles), dim3(C::WAVES * 64), 0, st, a);
     return hipGetLastError() == hipSuccess ? ACMIL_OK : ACMIL_ERR_LAUNCH;
 }
 
 template <int KIND, int DT> int ns_product(NsArgs& a, hipStream_t st) {
     // the largest tile that still gives most CUs work: larger tiles read less of LDS and L2 per flop
-    if (ns_tiles<NsM>(a, KIND) >= 200) return ns_go<NsM, 3, KIND, DT>(a, st);
+    if (ns_tiles<NsM>(a, KIND) >= 200) return ns_go<NsM, 2, KIND, DT>(a, st);
     if (ns_tiles<NsS>(a, KIND) >= 200) return ns_go<NsS, 2, KIND, DT>(a, st);
-    return ns_go<NsT, 6, KIND, DT>(a, st);
+    return ns_go<NsT, 4, KIND, DT>(a, st);
 }
 
 template <int DT> int ns_run(int count, const acmil_ortho_mat* mats, int steps, const float* co, float eps, char* ws, hipStream_t st) {
