@@ -38,9 +38,9 @@ static inline int mm_steps(const MmArgs& a) { return a.segs * ((((a.Kq > a.Kp) ?
 int mm_launch_fwd(const MmArgs& a, bool bf, int epi, bool dual, bool large, hipStream_t st);     // P, Q with K contiguous
 int mm_launch_dgrad(const MmArgs& a, bool bf, int epi, bool large, hipStream_t st);              // P with K strided
 int mm_launch_wgrad(const MmArgs& a, bool bf, int epi, bool large, hipStream_t st);              // both with K strided
-// few rows: y / h of M <= MM_ROWS_MAX rows straight from memory, any alignment of 2 bytes
-#define MM_ROWS_MAX 32
+// few rows: y / h of M <= ACMIL_FEW_ROWS rows straight from memory, any alignment of 2 bytes
 int mm_launch_rows(const MmArgs& a, bool bf, bool dual, hipStream_t st);
+int mm_rows_splits(int M, int cols, int K, bool dual);         // > 1: e.part receives the sums of each K range
 
 template <bool BF> struct MmEl;
 template <> struct MmEl<true> { typedef __bf16 T; typedef bf16x8 V; };

@@ -152,6 +152,16 @@ void aligned_pair(Ctx& c, Mat& a, Mat& b) {
 
 enum { FWD, DGRAD, WGRAD };
 
+void join(Ctx& c, const MmArgs& a, int epi) {
+    const dim3 g((unsigned)(((long long)a.M * (a.e.ldpart / 8) + 255) / 256));
+#define JOIN(B, E) hipLaunchKernelGGL((mm_join_kernel<B, E>), g, dim3(256), 0, c.st, a)
+    if (epi == MM_GATE) { if (c.bf) JOIN(true, MM_GATE); else JOIN(false, MM_GATE); }
+    else if (epi == MM_GATE_BWD) { if (c.bf) JOIN(true, MM_GATE_BWD); else JOIN(false, MM_GATE_BWD); }
+    else { if (c.bf) JOIN(true, MM_ACT); else JOIN(false, MM_ACT); }
+#undef JOIN
+    c.launched();
+}
+
 // One product: tile, K split, launch, join.
 void product(Ctx& c, int kind, MmArgs a, int epi) {
     const bool dual = epi == MM_GATE;
@@ -177,15 +187,7 @@ void product(Ctx& c, int kind, MmArgs a, int epi) {
         const int e = a.splits > 1 ? MM_PART : epi;
         c.rc = kind == FWD ? mm_launch_fwd(a, c.bf, e, dual, large, c.st) : kind == DGRAD ? mm_launch_dgrad(a, c.bf, e, large, c.st)
                                                                              : mm_launch_wgrad(a, c.bf, e, large, c.st);
-        if (a.splits > 1 && c.rc == ACMIL_OK) {
-            const dim3 g((unsigned)(((long long)a.M * (a.e.ldpart / 8) + 255) / 256));
-#define JOIN(B, E) hipLaunchKernelGGL((mm_join_kernel<B, E>), g, dim3(256), 0, c.st, a)
-            if (epi == MM_GATE) { if (c.bf) JOIN(true, MM_GATE); else JOIN(false, MM_GATE); }
-            else if (epi == MM_GATE_BWD) { if (c.bf) JOIN(true, MM_GATE_BWD); else JOIN(false, MM_GATE_BWD); }
-            else { if (c.bf) JOIN(true, MM_ACT); else JOIN(false, MM_ACT); }
-#undef JOIN
-            c.launched();
-        }
+        if (a.splits > 1 && c.rc == ACMIL_OK) join(c, a, epi);
     }
     c.ar.off = mark;                                                 // the partial sums are dead behind the join: stream order
 }
@@ -231,8 +233,18 @@ bool same_dtype_ok(int dtype) { return dtype == ACMIL_DTYPE_F16 || dtype == ACMI
 bool act_ok(int act) { return act >= ACMIL_ACT_NONE && act <= ACMIL_ACT_SIGMOID; }
 bool ld_ok(const void* p, long long ld, int cols) { return !p || (ld >= 0 && ld <= MAX_LD && (ld >= cols || ld == 0)); }
 
-void few_rows(Ctx& c, const MmArgs& a, bool dual) {
-    if (c.go()) c.rc = mm_launch_rows(a, c.bf, dual, c.st);
+void few_rows(Ctx& c, MmArgs a, bool dual) {
+    const size_t mark = c.ar.off;
+    a.splits = mm_rows_splits(a.M, a.e.npad, a.Kq, dual);
+    if (a.splits > 1) {
+        a.e.ldpart = r8(a.e.npad);
+        a.e.part = (float*)c.ar.take((size_t)a.splits * (dual ? 2 : 1) * a.M * a.e.ldpart * 4);
+    }
+    if (c.room() && c.go()) {
+        c.rc = mm_launch_rows(a, c.bf, dual, c.st);
+        if (a.splits > 1 && c.rc == ACMIL_OK) join(c, a, dual ? MM_GATE : MM_ACT);
+    }
+    c.ar.off = mark;
 }
 
 int linear_check(const acmil_linear_args* a, bool backward) {
@@ -254,7 +266,7 @@ int linear_check(const acmil_linear_args* a, bool backward) {
 
 int linear_fwd(const acmil_linear_args& a, Ctx& c) {
     Mat x{a.x, a.ldx, a.M, a.K}, w{a.W, a.ldw, a.N, a.K};
-    const bool few = a.M <= MM_ROWS_MAX;
+    const bool few = a.M <= ACMIL_FEW_ROWS;
     if (!few) { x = aligned(c, x); w = aligned(c, w); }
     MmArgs p = operands(x, w, a.M, a.N, x.cols, w.cols);
     output(p, a.y, a.ldy, a.bias, a.res, a.ldr);
@@ -314,7 +326,7 @@ int ffn_check(const acmil_ffn_args* a, bool backward) {
 
 int ffn_fwd(const acmil_ffn_args& a, Ctx& c) {
     const int F8 = r8(a.F);
-    const bool few = a.M <= MM_ROWS_MAX;
+    const bool few = a.M <= ACMIL_FEW_ROWS;
     Mat x{a.x, a.ldx, a.M, a.D}, wg{a.Wg, a.ldwg, a.F, a.D}, wu{a.Wu, a.ldwu, a.F, a.D}, wd{a.Wd, a.ldwd, a.D, a.F};
     if (!few) { x = aligned(c, x); aligned_pair(c, wg, wu); wd = aligned(c, wd); }
     else if (wg.ld != wu.ld) aligned_pair(c, wg, wu);                // one leading dimension for both
@@ -373,19 +385,21 @@ int ffn_bwd(const acmil_ffn_args& a, Ctx& c) {
     return c.rc;
 }
 
+const size_t NOTHING = 256;      // what a call that takes no workspace answers to the query (0 = refused)
 template <class A> size_t need(const A* a, int rc, int (*f)(const A&, Ctx&)) {
     if (rc != ACMIL_OK) return 0;
     Arena ar{nullptr, 0};
     Ctx c{ar, a->dtype == ACMIL_DTYPE_BF16, nullptr};
     f(*a, c);
-    return (ar.peak + 255 + 256) & ~(size_t)255;
+    return ((ar.peak + 255) & ~(size_t)255) + NOTHING;
 }
 template <class A> int go(const A* a, int rc, int (*f)(const A&, Ctx&), void* ws, size_t bytes, void* stream) {
     if (rc != ACMIL_OK) return rc;
-    if (!ws) return ACMIL_ERR_NULL;
     if (((size_t)ws & 255) != 0) return ACMIL_ERR_SHAPE;
-    if (bytes < need(a, rc, f)) return ACMIL_ERR_SHAPE;              // before anything is launched
-    Arena ar{(char*)ws, bytes};
+    const size_t want = need(a, rc, f);                              // before anything is launched
+    if (want > NOTHING && !ws) return ACMIL_ERR_NULL;
+    if (want > NOTHING && bytes < want) return ACMIL_ERR_SHAPE;
+    Arena ar{ws ? (char*)ws : (char*)256, bytes};                    // (nothing is taken from a workspace that is not needed)
     Ctx c{ar, a->dtype == ACMIL_DTYPE_BF16, (hipStream_t)stream};
     return f(*a, c);
 }

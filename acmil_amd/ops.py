@@ -959,19 +959,20 @@ def linear_f16x3(x: torch.Tensor, packed: torch.Tensor, n_out: int, bias: Option
 # ---------------------------------------------------------------------------------------------------------------------
 _HALF = (torch.float16, torch.bfloat16)
 _MAX_ROWS, _MAX_DIM, _MAX_LD = (1 << 31) - 1, 1 << 22, 1 << 22
+_NO_WORKSPACE_ROWS = 4     # acmil_linear_act of at most so many rows takes no workspace
 
 
-def _half_inputs(name: str, *ts: Optional[torch.Tensor]) -> torch.device:
+def _half_inputs(name: str, first: torch.Tensor, *others: Optional[torch.Tensor]) -> torch.device:
     """One CUDA device and one 16-bit type for every tensor of the call."""
-    _need_cuda(*ts)
-    first = ts[0]
-    if first.dtype not in _HALF:
-        raise RuntimeError("acmil_amd.%s: fp16 or bf16 tensors (got %s); fp32 layers are acmil_amd.autograd.linear / ops.linear_f16x3" % (name, first.dtype))
-    for t in ts:
-        if t is not None and (t.dtype != first.dtype or t.device != first.device):
-            raise RuntimeError("acmil_amd.%s: all tensors must have one type and one device (%s on %s and %s on %s)"
-                               % (name, first.dtype, first.device, t.dtype, t.device))
-    return first.device
+    dt, dev = first.dtype, first.device
+    for t in others:
+        if t is not None and (t.dtype != dt or t.device != dev):
+            _need_cuda(first, t)
+            raise RuntimeError("acmil_amd.%s: all tensors must have one type and one device (%s on %s and %s on %s)" % (name, dt, dev, t.dtype, t.device))
+    if dev.type != "cuda" or dt not in _HALF:
+        _need_cuda(first)
+        raise RuntimeError("acmil_amd.%s: fp16 or bf16 tensors (got %s); fp32 layers are acmil_amd.autograd.linear / ops.linear_f16x3" % (name, dt))
+    return dev
 
 
 def _act_id(name: str, act: str) -> int:
@@ -983,50 +984,49 @@ def _act_id(name: str, act: str) -> int:
 def _rows16(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
     """t [..., C] as a matrix the library can address: (2-D tensor with unit inner stride, leading dimension).  Row strides are kept
     (0 = every row the same); anything else -- a strided inner dimension, overlapping rows -- is copied once."""
-    t = t.detach()
-    c = t.shape[-1]
     if t.dim() != 2:
-        t = t.reshape(-1, c)
-    ld = t.stride(0) if t.shape[0] > 1 else c
-    if (c > 1 and t.stride(1) != 1) or (ld != 0 and ld < c) or ld > _MAX_LD:
-        t = t.contiguous()
+        t = t.detach().reshape(-1, t.shape[-1])
+    rows, c = t.shape
+    ld, inner = t.stride()
+    if rows <= 1:
         ld = c
-    return t, ld
+    if (inner == 1 or c == 1) and (ld >= c or ld == 0) and ld <= _MAX_LD:
+        return t, ld
+    return t.detach().contiguous(), c
 
 
 def _vec16(name: str, what: str, t: Optional[torch.Tensor], n: int) -> Optional[torch.Tensor]:
     if t is None:
         return None
-    if t.shape != (n,):
+    if t.dim() != 1 or t.shape[0] != n:
         raise RuntimeError("acmil_amd.%s: %s must be [%d], got %s" % (name, what, n, tuple(t.shape)))
-    return t.detach().contiguous()
+    return t if t.stride(0) == 1 else t.detach().contiguous()
 
 
-def _half_call(name: str, args, device: torch.device) -> None:
+def _half_call(lib, name: str, args, device: torch.device, may_need: bool = True) -> None:
     """Workspace query + call of a C entry that takes one argument block, on the tensors' device and its current stream."""
-    lib = _lib.load()
-    if device.index is not None and device.index != torch.cuda.current_device():
+    if device.index != torch._C._cuda_getDevice():
         with torch.cuda.device(device):
-            return _half_call(name, args, device)
-    ref = ctypes.byref(args)
-    need = getattr(lib, name + "_workspace_bytes")(ref)
-    if need == 0:
-        raise RuntimeError("%s: the arguments are refused (a dimension or leading dimension is out of range)" % name)
-    ws = torch.empty(need, dtype=torch.uint8, device=device)
-    _lib.check(getattr(lib, name)(ref, ws.data_ptr(), need, _stream()), name)
+            return _half_call(lib, name, args, device, may_need)
+    ref, ws, need = ctypes.byref(args), None, 0
+    if may_need:
+        need = getattr(lib, name + "_workspace_bytes")(ref)
+        if need == 0:
+            raise RuntimeError("%s: the arguments are refused (a dimension or leading dimension is out of range)" % name)
+        ws = torch.empty(need, dtype=torch.uint8, device=device)
+    _lib.check(getattr(lib, name)(ref, None if ws is None else ws.data_ptr(), need, torch._C._cuda_getCurrentRawStream(device.index)), name)
 
 
 def _linear_args(name: str, x: torch.Tensor, weight: torch.Tensor, act: str):
     if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or 0 in weight.shape:
         raise RuntimeError("acmil_amd.%s: x [..., in] and weight [out, in] expected, got %s and %s" % (name, tuple(x.shape), tuple(weight.shape)))
-    if max(weight.shape) > _MAX_DIM or x.numel() // weight.shape[1] > _MAX_ROWS:
+    N, K = weight.shape
+    x2, ldx = _rows16(x)
+    w2, ldw = _rows16(weight)
+    M = x2.shape[0]
+    if N > _MAX_DIM or K > _MAX_DIM or M > _MAX_ROWS:
         raise RuntimeError("acmil_amd.%s: at most %d features and %d rows" % (name, _MAX_DIM, _MAX_ROWS))
-    a = _lib.LinearArgs(dtype=_DT[x.dtype], act=_act_id(name, act))
-    x2, a.ldx = _rows16(x)
-    w2, a.ldw = _rows16(weight)
-    a.M, a.K, a.N = x2.shape[0], x2.shape[1], w2.shape[0]
-    a.x, a.W = x2.data_ptr(), w2.data_ptr()
-    return a, x2, w2
+    return _lib.LinearArgs(_DT[x.dtype], _act_id(name, act), M, K, N, x2.data_ptr(), ldx, w2.data_ptr(), ldw), x2, w2
 
 
 def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, act: str = "none",
@@ -1037,19 +1037,23 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
     ([rows, round8(out)]), what linear_act_bwd wants.  No gradient is recorded (acmil_amd.autograd.linear_act is the differentiable form)."""
     dev = _half_inputs("linear_act", x, weight, bias, residual)
     a, x2, w2 = _linear_args("linear_act", x, weight, act)
-    shape = tuple(x.shape[:-1]) + (a.N,)
-    b = _vec16("linear_act", "bias", bias, a.N)
-    if residual is not None and tuple(residual.shape) != shape:
-        raise RuntimeError("acmil_amd.linear_act: residual must be %s, got %s" % (shape, tuple(residual.shape)))
+    M, N = a.M, a.N
+    shape = x.shape[:-1] + (N,)
+    b = _vec16("linear_act", "bias", bias, N)
+    if residual is not None and residual.shape != shape:
+        raise RuntimeError("acmil_amd.linear_act: residual must be %s, got %s" % (tuple(shape), tuple(residual.shape)))
     y = torch.empty(shape, dtype=x.dtype, device=dev)
-    pre = torch.empty(a.M, (a.N + 7) // 8 * 8, dtype=torch.float32, device=dev) if keep_pre else None
-    if a.M > 0:
-        a.y, a.ldy, a.bias, a.pre = y.data_ptr(), a.N, _ptr(b), _ptr(pre)
-        r2 = None
+    pre = torch.empty(M, (N + 7) // 8 * 8, dtype=torch.float32, device=dev) if keep_pre else None
+    if M > 0:
+        a.y, a.ldy = y.data_ptr(), N
+        if b is not None:
+            a.bias = b.data_ptr()
+        if keep_pre:
+            a.pre = pre.data_ptr()
         if residual is not None:
             r2, a.ldr = _rows16(residual)
             a.res = r2.data_ptr()
-        _half_call("acmil_linear_act", a, dev)
+        _half_call(_lib.load(), "acmil_linear_act", a, dev, may_need=M > _NO_WORKSPACE_ROWS)
     return (y, pre) if keep_pre else y
 
 
@@ -1071,7 +1075,7 @@ def linear_act_bwd(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, pre:
     if a.M > 0 and any(need):
         dy2, a.lddy = _rows16(dy)
         a.dy, a.pre, a.dx, a.dW, a.db = dy2.data_ptr(), _ptr(pre), _ptr(dx), _ptr(dw), _ptr(db)
-        _half_call("acmil_linear_act_bwd", a, dev)
+        _half_call(_lib.load(), "acmil_linear_act_bwd", a, dev)
     return dx, dw, db
 
 
@@ -1081,15 +1085,15 @@ def _ffn_args(name: str, x, w_gate, w_up, w_down, act: str):
         raise RuntimeError("acmil_amd.%s: x [..., D], w_gate and w_up [F, D], w_down [D, F] expected, got %s, %s, %s, %s"
                            % (name, tuple(x.shape), tuple(w_gate.shape), tuple(w_up.shape), tuple(w_down.shape)))
     F, D = w_gate.shape
-    if D > _MAX_DIM or F > _MAX_DIM // 2 or x.numel() // D > _MAX_ROWS:
+    x2, ldx = _rows16(x)
+    g2, ldg = _rows16(w_gate)
+    u2, ldu = _rows16(w_up)
+    d2, ldd = _rows16(w_down)
+    M = x2.shape[0]
+    if D > _MAX_DIM or F > _MAX_DIM // 2 or M > _MAX_ROWS:
         raise RuntimeError("acmil_amd.%s: at most %d features, %d hidden features and %d rows" % (name, _MAX_DIM, _MAX_DIM // 2, _MAX_ROWS))
-    a = _lib.FfnArgs(dtype=_DT[x.dtype], act=_act_id(name, act), D=D, F=F)
-    x2, a.ldx = _rows16(x)
-    g2, a.ldwg = _rows16(w_gate)
-    u2, a.ldwu = _rows16(w_up)
-    d2, a.ldwd = _rows16(w_down)
-    a.M, a.x, a.Wg, a.Wu, a.Wd = x2.shape[0], x2.data_ptr(), g2.data_ptr(), u2.data_ptr(), d2.data_ptr()
-    return a, (x2, g2, u2, d2)
+    return _lib.FfnArgs(_DT[x.dtype], _act_id(name, act), M, D, F, x2.data_ptr(), ldx, g2.data_ptr(), ldg, u2.data_ptr(), ldu, d2.data_ptr(),
+                        ldd), (x2, g2, u2, d2)
 
 
 def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, b_gate: Optional[torch.Tensor] = None,
@@ -1113,11 +1117,13 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
                  torch.empty(a.M, f8, dtype=x.dtype, device=dev))
         a.g, a.u, a.h = (t.data_ptr() for t in saved)
     if a.M > 0:
-        a.y, a.ldy, a.bg, a.bu, a.bd = y.data_ptr(), a.D, _ptr(bg), _ptr(bu), _ptr(bd)
+        a.y, a.ldy = y.data_ptr(), a.D
+        if bg is not None or bu is not None or bd is not None:
+            a.bg, a.bu, a.bd = _ptr(bg), _ptr(bu), _ptr(bd)
         if residual is not None:
             r2, a.ldr = _rows16(residual)
             a.res = r2.data_ptr()
-        _half_call("acmil_gated_ffn", a, dev)
+        _half_call(_lib.load(), "acmil_gated_ffn", a, dev)
     return (y, saved) if keep else y
 
 
@@ -1145,7 +1151,7 @@ def gated_ffn_bwd(dy: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w_up:
         dy2, a.lddy = _rows16(dy)
         a.dy, a.g, a.u, a.h = dy2.data_ptr(), g.data_ptr(), u.data_ptr(), h.data_ptr()
         a.dx, a.dWgu, a.dWd, a.dbgu, a.dbd = _ptr(dx), _ptr(dgu), _ptr(dd), _ptr(bgu), _ptr(bd)
-        _half_call("acmil_gated_ffn_bwd", a, dev)
+        _half_call(_lib.load(), "acmil_gated_ffn_bwd", a, dev)
     F = a.F
     return (dx, None if dgu is None else dgu[:F], None if dgu is None else dgu[f8:f8 + F], dd,
             None if bgu is None else bgu[:F], None if bgu is None else bgu[f8:f8 + F], bd)

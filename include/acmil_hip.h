@@ -598,7 +598,8 @@ int acmil_adamw_step_peer(float* params, float* exp_avg, float* exp_avg_sq, long
  * All tensors of one call have ONE type (dtype: ACMIL_DTYPE_F16 / _BF16); products accumulate in fp32, bias, activation, gate and
  * residual are applied in fp32, and every output is rounded once.  Matrices are row-major with unit inner stride; a leading dimension
  * (in elements) may exceed the row, or be 0 (every row the same); base addresses need 2-byte alignment only.  Matrices whose rows do
- * not start on 16 bytes or whose length is no multiple of 8 are copied into the workspace first, except in calls of at most 32 rows.
+ * not start on 16 bytes or whose length is no multiple of 8 are copied into the workspace first, except in forward calls of at most
+ * ACMIL_FEW_ROWS rows.
  *   acmil_linear_act      y [M,N] = act(x W^T + bias) + res        x [M,K], W [N,K], bias [N] or NULL, res [M,N] or NULL (ldr)
  *     pre: NULL, or fp32 [M][round8(N)] (16-byte aligned) that receives x W^T + bias for the backward (act != NONE needs it)
  *   acmil_linear_act_bwd  dz = dy act'(pre); dx [M,K] = dz W, dW [N,K] = dz^T x, db [N] = column sums of dz (each may be NULL; dense);
@@ -612,8 +613,10 @@ int acmil_adamw_step_peer(float* params, float* exp_avg, float* exp_avg_sq, long
  * Results are reproducible bit for bit (no atomics; K splits are joined in a fixed order).
  * workspace: acmil_*_workspace_bytes(args) bytes, 256-byte aligned, contents arbitrary, dead when the call's work is done.  The
  * query reads the same argument block (base addresses included: they decide about copies); 0 = the arguments are refused.
+ * acmil_linear_act of at most 4 rows needs no workspace (NULL).
  * 1 <= M; 1 <= K, N, D <= 2^22, F <= 2^21; leading dimensions <= 2^22.
  * ------------------------------------------------------------------------------------------- */
+#define ACMIL_FEW_ROWS 32     /* acmil_linear_act and acmil_gated_ffn of at most so many rows read the weights straight from memory */
 #define ACMIL_ACT_NONE 0
 #define ACMIL_ACT_RELU 1
 #define ACMIL_ACT_SILU 2      /* z sigmoid(z) */

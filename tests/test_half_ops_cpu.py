@@ -32,10 +32,10 @@ def test_linear_entry_refuses(change, code):
 
 def test_entries_refuse_missing_pieces():
     lib = _lib.load()
-    good = dict(dtype=2, act=2, M=40, K=16, N=8, x=4096, W=4096, ldx=16, ldw=16, y=4096, ldy=8)
+    good = dict(dtype=2, act=2, M=40, K=4096, N=8, x=4096, W=4096, ldx=4096, ldw=4096, y=4096, ldy=8)      # (K is split: needs a workspace)
     a = _lib.LinearArgs(**good)
     need = lib.acmil_linear_act_workspace_bytes(ctypes.byref(a))
-    assert need >= 256
+    assert need > 256
     assert lib.acmil_linear_act(ctypes.byref(a), None, need, None) == -3                 # no workspace
     assert lib.acmil_linear_act(ctypes.byref(a), 4097, need, None) == -1                 # not on 256 bytes
     assert lib.acmil_linear_act(ctypes.byref(a), 4096, need - 1, None) == -1             # too small
