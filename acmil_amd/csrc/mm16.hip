@@ -162,6 +162,21 @@ void join(Ctx& c, const MmArgs& a, int epi) {
     c.launched();
 }
 
+// How many ways to split K of a product of 128 x 128 tiles.  A step of one tile takes about 0.55 us alone on its CU and 1.0 us beside
+// another; a split costs a join launch and 8 bytes of partial sums per output and part, written and read at about 4 TB/s.  Without the
+// second term (split until 512 workgroups) 2000 x 768 x 768 took 20.2 us against 11.1, without a split at all 64 x 4096 x 4096 37 against 14.
+int mm_splits(long long tiles, int steps, double outputs) {
+    int best = 1;
+    double least = 1e30;
+    for (int s = 1; s <= 64 && s * 4 <= (steps > 4 ? steps : 4); ++s) {
+        const long long wgs = tiles * s, rounds = (wgs + 511) / 512, rest = wgs - 512 * (rounds - 1);
+        const double step = (rounds - 1) * 1.0 + (rest > 256 ? 1.0 : 0.55);
+        const double us = ((steps + s - 1) / s) * step + (s > 1 ? 2.5 + s * outputs * 8.0 / 4e6 : 0.0);
+        if (us < least) { least = us; best = s; }
+    }
+    return best;
+}
+
 // One product: tile, K split, launch, join.
 void product(Ctx& c, int kind, MmArgs a, int epi) {
     const bool dual = epi == MM_GATE;
@@ -174,10 +189,7 @@ void product(Ctx& c, int kind, MmArgs a, int epi) {
     a.ntm = (a.M + b - 1) / b;
     a.ntn = (n_eff + b - 1) / b;
     const long long tiles = (long long)a.ntm * a.ntn;
-    // few tiles: split K so that the workgroups fill the chip twice over, at least 4 steps each
-    long long sp = large ? 1 : 512 / tiles;
-    if (sp > steps / 4) sp = steps / 4;
-    a.splits = (int)(sp < 1 ? 1 : sp > 64 ? 64 : sp);
+    a.splits = large ? 1 : mm_splits(tiles, steps, (double)a.M * r8(a.e.npad) * (dual ? 2 : 1));
     const size_t mark = c.ar.off;
     if (a.splits > 1) {
         a.e.ldpart = r8(a.e.npad);
