@@ -10,6 +10,8 @@ enum { MM_KC = 0, MM_KS = 1 };   // operand element (row, k) lies at row * ld + 
 // MM_GATE_BWD: v = dh -> dg = dh u act'(g), du = dh act(g).  MM_PART: raw fp32 sums of one K range for mm_join.
 enum { MM_ACT = 0, MM_GATE = 1, MM_GATE_BWD = 2, MM_PART = 3 };
 
+enum { MM_S = 0, MM_L = 1, MM_D = 2 };   // tile configurations of mm16_kernel.h
+
 struct MmEpi {
     int act, vec;                      // vec: every row that is touched starts on 16 bytes
     const void *bias, *bias2;          // [N] in the operands' type, or null (bias2: of the second factor)
@@ -35,9 +37,9 @@ struct MmArgs {
 
 // K steps of mm16_kernel.h
 static inline int mm_steps(const MmArgs& a) { return a.segs * ((((a.Kq > a.Kp) ? a.Kq : a.Kp) + 63) / 64); }
-int mm_launch_fwd(const MmArgs& a, bool bf, int epi, bool dual, bool large, hipStream_t st);     // P, Q with K contiguous
-int mm_launch_dgrad(const MmArgs& a, bool bf, int epi, bool large, hipStream_t st);              // P with K strided
-int mm_launch_wgrad(const MmArgs& a, bool bf, int epi, bool large, hipStream_t st);              // both with K strided
+int mm_launch_fwd(const MmArgs& a, bool bf, int epi, bool dual, int cfg, hipStream_t st);     // P, Q with K contiguous
+int mm_launch_dgrad(const MmArgs& a, bool bf, int epi, int cfg, hipStream_t st);              // P with K strided
+int mm_launch_wgrad(const MmArgs& a, bool bf, int epi, int cfg, hipStream_t st);              // both with K strided
 // few rows: y / h of M <= ACMIL_FEW_ROWS rows straight from memory, any alignment of 2 bytes
 int mm_launch_rows(const MmArgs& a, bool bf, bool dual, hipStream_t st);
 int mm_rows_splits(int M, int cols, int K, bool dual);         // > 1: e.part receives the sums of each K range

@@ -196,9 +196,9 @@ void product(Ctx& c, int kind, MmArgs a, int epi) {
         a.e.part = (float*)c.ar.take((size_t)a.splits * (dual ? 2 : 1) * a.M * a.e.ldpart * 4);
     }
     if (c.room() && c.go()) {
-        const int e = a.splits > 1 ? MM_PART : epi;
-        c.rc = kind == FWD ? mm_launch_fwd(a, c.bf, e, dual, large, c.st) : kind == DGRAD ? mm_launch_dgrad(a, c.bf, e, large, c.st)
-                                                                             : mm_launch_wgrad(a, c.bf, e, large, c.st);
+        const int e = a.splits > 1 ? MM_PART : epi, cfg = large ? MM_L : tiles * a.splits <= 256 ? MM_D : MM_S;
+        c.rc = kind == FWD ? mm_launch_fwd(a, c.bf, e, dual, cfg, c.st) : kind == DGRAD ? mm_launch_dgrad(a, c.bf, e, cfg, c.st)
+                                                                             : mm_launch_wgrad(a, c.bf, e, cfg, c.st);
         if (a.splits > 1 && c.rc == ACMIL_OK) join(c, a, epi);
     }
     c.ar.off = mark;                                                 // the partial sums are dead behind the join: stream order

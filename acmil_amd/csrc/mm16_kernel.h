@@ -5,8 +5,8 @@
 // dW = dz^T x: P = x (KS), Q = dz (KS).  DUAL multiplies the same Q by two P (gate and up projection) so that one wave holds both
 // factors of an output element in its accumulators and the product needs no second pass.
 //
-// Layout.  A K step is 64 wide.  Tiles travel global -> LDS by 16-byte LDS-DMA (no registers) through a ring of two stages, one barrier
-// a step.  The LDS image is linear in the DMA's lane order, so bank
+// Layout.  A K step is 64 wide.  Tiles travel global -> LDS by 16-byte LDS-DMA (no registers) through a ring, one barrier a
+// step.  The LDS image is linear in the DMA's lane order, so bank
 // conflicts are avoided by permuting which 16-byte chunk of its row each LANE FETCHES.  K-strided tiles lie in LDS as they lie in
 // memory ([k][row]) and are read by ds_read_b64_tr_b16, which hands every lane four consecutive k of its row: no transposed copy of
 // an operand is ever made.  P feeds the A side of the instruction: a lane then owns 4 consecutive COLUMNS of an output row.
@@ -38,10 +38,13 @@ template <int BM_, int BN_, int WAVES_, int WN_> struct MmGeom {
     static constexpr int TM = BM / (WAVES / WN), TN = BN / WN, MT = TM / 16, NT = TN / 16;
     static constexpr int QB = BM * 128, PB = BN * 128;
 };
-// LARGE: one 8-wave workgroup per CU, else two 4-wave workgroups per CU; either way all 160 KB of LDS
-template <bool LARGE> struct MmCfg;
-template <> struct MmCfg<true> : MmGeom<256, 256, 8, 4> {};
-template <> struct MmCfg<false> : MmGeom<128, 128, 4, 2> {};
+// MM_L: one 8-wave workgroup per CU.  MM_S: two 4-wave workgroups per CU.  MM_D: one 8-wave workgroup per CU that looks three steps ahead
+// instead of one -- alone on its CU a workgroup of MM_S waits a memory latency (about 1 us) for every second step.  D: steps of the ring, of
+// 2 D + 1 slots: all 160 KB of LDS or nearly.
+template <int CFG> struct MmCfg;
+template <> struct MmCfg<MM_L> : MmGeom<256, 256, 8, 4> { static constexpr int D = 2, PER_SIMD = 2; };
+template <> struct MmCfg<MM_S> : MmGeom<128, 128, 4, 2> { static constexpr int D = 2, PER_SIMD = 2; };
+template <> struct MmCfg<MM_D> : MmGeom<128, 128, 8, 2> { static constexpr int D = 4, PER_SIMD = 2; };
 
 __device__ __forceinline__ unsigned mm_lds_addr(const void* p) { return (unsigned)(size_t)(const __attribute__((address_space(3))) void*)p; }
 
@@ -117,11 +120,11 @@ template <bool BF> __device__ __forceinline__ f32x4 mm_mfma(s16x8 a, s16x8 b, f3
     else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-template <bool BF, int PK, int QK, int EPI, bool DUAL, bool LARGE>
-__global__ __launch_bounds__(MmCfg<LARGE>::WAVES * 64, 2) void mm16_kernel(MmArgs a) {
-    using C = MmCfg<LARGE>;
+template <bool BF, int PK, int QK, int EPI, bool DUAL, int CFG>
+__global__ __launch_bounds__(MmCfg<CFG>::WAVES * 64, MmCfg<CFG>::PER_SIMD) void mm16_kernel(MmArgs a) {
+    using C = MmCfg<CFG>;
     constexpr int MT = C::MT, NT = C::NT;
-    constexpr int SLOT = C::QB, SLOTS = 5;                           // half a stage: one operand of one K step
+    constexpr int SLOT = C::QB, D = C::D, SLOTS = 2 * D + 1;                           // half a stage: one operand of one K step
     static_assert(C::QB == C::PB, "either operand fits any slot");
     __shared__ __attribute__((aligned(128))) char smem[SLOTS * SLOT];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -200,11 +203,11 @@ __global__ __launch_bounds__(MmCfg<LARGE>::WAVES * 64, 2) void mm16_kernel(MmArg
     fq.init(lane, wm * C::TM);
     fp.init(lane, wn * (DUAL ? C::TN / 2 : C::TN));
 
-    // The ring has five slots for Q_0 P_0 Q_1 P_1 Q_2 ...  A step is two pieces of 32 k.  A piece goes row tile by row tile: NT matrix
+    // The ring has 2 D + 1 slots for Q_0 P_0 Q_1 P_1 Q_2 ...  A step is two pieces of 32 k.  A piece goes row tile by row tile: NT matrix
     // instructions, then the row fragment just used is read again for the next piece (the column fragments, which every row tile needs,
     // have two register sets).  Between the pieces of step t a wave has read all it needs of Q_t and P_t, and its share of Q_(t+1) and
-    // P_(t+1) has landed: behind the one barrier of the step the first fragments of step t + 1 are read.  Q_(t+2) is fetched during the
-    // first piece, into the slot that was free, and P_(t+2) during the second, into that of Q_t.  Fetches are spread over the step because
+    // P_(t+1) has landed: behind the one barrier of the step the first fragments of step t + 1 are read.  Q_(t+D) is fetched during the
+    // first piece, into the slot that was free, and P_(t+D) during the second, into that of Q_t.  Fetches are spread over the step because
     // one that finds the address unit busy holds its wave up, with its matrix instructions: sent out in one burst behind the barrier
     // they cost 18 % more cycles.
     s16x8 p[2][NT], q[MT];
@@ -236,20 +239,20 @@ __global__ __launch_bounds__(MmCfg<LARGE>::WAVES * 64, 2) void mm16_kernel(MmArg
                 __builtin_amdgcn_sched_barrier(0);
             });
         };
-        mm_for<0, 2>([&](auto i) MM_INLINE {
+        mm_for<0, D>([&](auto i) MM_INLINE {
             const Half hq = half_of(t0 + i, 2 * i, true), hp = half_of(t0 + i, 2 * i + 1, false);
             mm_for<0, NI>([&](auto d) MM_INLINE { fetch_q(hq, d, tail); });
             mm_for<0, NI>([&](auto d) MM_INLINE { fetch_p(hp, d, tail); });
         });
-        mm_wait_dma<2 * NI>();
+        mm_wait_dma<(2 * D - 2) * NI>();
         ga_lds_barrier();
-        int qs = 0, ps = 1, free = 4;                                // slots of Q_t, P_t and the one that Q_(t+2) goes to
+        int qs = 0, ps = 1, free = SLOTS - 1;                        // slots of Q_t, P_t and the one that Q_(t+D) goes to
         mm_for<0, NT>([&](auto f) MM_INLINE { read_p(ring + SLOT, std::integral_constant<int, 0>{}, f); });
         mm_for<0, MT>([&](auto f) MM_INLINE { read_q(ring, std::integral_constant<int, 0>{}, f); });
         for (int t = t0; t < t1; ++t) {
-            const Half hq = half_of(t + 2, free, true), hp = half_of(t + 2, qs, false);
+            const Half hq = half_of(t + D, free, true), hp = half_of(t + D, qs, false);
             piece(std::integral_constant<int, 0>{}, ring + qs * SLOT, ring + ps * SLOT, hq);
-            mm_wait_dma<NI>();                                       // Q_(t+2) may still be on its way
+            mm_wait_dma<(2 * D - 3) * NI>();                         // younger steps may still be on their way
             ga_lds_barrier();
             free = ps;
             qs = qs >= SLOTS - 2 ? qs + 2 - SLOTS : qs + 2;
@@ -305,11 +308,15 @@ __global__ __launch_bounds__(MmCfg<LARGE>::WAVES * 64, 2) void mm16_kernel(MmArg
     }
 }
 
-template <bool BF, int PK, int QK, int EPI, bool DUAL, bool LARGE> static inline int mm_go(const MmArgs& a, hipStream_t st) {
-    hipLaunchKernelGGL((mm16_kernel<BF, PK, QK, EPI, DUAL, LARGE>), dim3(a.ntm * a.ntn, a.splits), dim3(MmCfg<LARGE>::WAVES * 64), 0, st, a);
+template <bool BF, int PK, int QK, int EPI, bool DUAL, int CFG> static inline int mm_go(const MmArgs& a, hipStream_t st) {
+    hipLaunchKernelGGL((mm16_kernel<BF, PK, QK, EPI, DUAL, CFG>), dim3(a.ntm * a.ntn, a.splits), dim3(MmCfg<CFG>::WAVES * 64), 0, st, a);
     return hipGetLastError() == hipSuccess ? ACMIL_OK : ACMIL_ERR_LAUNCH;
 }
-template <int PK, int QK, int EPI, bool DUAL> static inline int mm_go_any(const MmArgs& a, bool bf, bool large, hipStream_t st) {
-    if (bf) return large ? mm_go<true, PK, QK, EPI, DUAL, true>(a, st) : mm_go<true, PK, QK, EPI, DUAL, false>(a, st);
-    return large ? mm_go<false, PK, QK, EPI, DUAL, true>(a, st) : mm_go<false, PK, QK, EPI, DUAL, false>(a, st);
+template <bool BF, int PK, int QK, int EPI, bool DUAL> static inline int mm_go_cfg(const MmArgs& a, int cfg, hipStream_t st) {
+    // (K is never split where the large tiles fill the chip)
+    if constexpr (EPI != MM_PART) if (cfg == MM_L) return mm_go<BF, PK, QK, EPI, DUAL, MM_L>(a, st);
+    return cfg == MM_D ? mm_go<BF, PK, QK, EPI, DUAL, MM_D>(a, st) : mm_go<BF, PK, QK, EPI, DUAL, MM_S>(a, st);
+}
+template <int PK, int QK, int EPI, bool DUAL> static inline int mm_go_any(const MmArgs& a, bool bf, int cfg, hipStream_t st) {
+    return bf ? mm_go_cfg<true, PK, QK, EPI, DUAL>(a, cfg, st) : mm_go_cfg<false, PK, QK, EPI, DUAL>(a, cfg, st);
 }

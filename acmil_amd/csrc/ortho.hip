@@ -138,14 +138,18 @@ template <int DT> __global__ __launch_bounds__(256) void ns_split_kernel(NsArgs 
 
 // One product tile.  As in mm16_kernel.h, with 32 pairs a step and so one piece a step: the fragments of step t + 1 are read while those of
 // step t multiply, and behind the barrier in front of step t both slots of its stage are free.  D steps are in flight or being read.
-template <class C, int D, int KIND, int DT>
-__global__ __launch_bounds__(C::WAVES * 64) void ns_kernel(NsArgs a) {
+// KG groups of waves take a share of the steps each, with a ring of their own, and add up in LDS: where there are fewer tiles than CUs, one
+// group spends most of a step waiting for its barrier and its fragments.
+template <class C, int D, int KG, int KIND, int DT>
+__global__ __launch_bounds__(C::WAVES * KG * 64) void ns_kernel(NsArgs a) {
     constexpr int MT = C::MT, NT = C::NT;
     constexpr int SLOT = C::QB, SLOTS = 2 * D + 1;
     static_assert(C::QB == C::PB && D >= 2, "either operand fits any slot");
-    __shared__ __attribute__((aligned(128))) char smem[SLOTS * SLOT];
-    static_assert(C::WAVES * 32 * 36 * 4 <= SLOTS * SLOT, "room for the turned tiles");
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    __shared__ __attribute__((aligned(128))) char smem[KG * SLOTS * SLOT];
+    static_assert(MT % 2 == 0 && C::WAVES * 32 * 20 * 4 <= SLOTS * SLOT, "room for the turned tiles");
+    static_assert((KG - 1) * C::WAVES * MT * NT * 1024 <= KG * SLOTS * SLOT, "room for the other groups' sums");
+    const int lane = threadIdx.x & 63, wave_all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int group = wave_all / C::WAVES, wave = wave_all % C::WAVES;
     const int wm = wave / C::WN, wn = wave % C::WN;
     int blk;
     {   // workgroup b runs on XCD b % 8: every XCD takes one contiguous run of tiles
@@ -180,12 +184,14 @@ __global__ __launch_bounds__(C::WAVES * 64) void ns_kernel(NsArgs a) {
     lp.init(wave, lane, ldk, n0, N);
     qp += m0 * ldk;
     pp += n0 * ldk;
-    const int T = ns_r32(K) / 32;
-    const unsigned smem0 = mm_lds_addr(smem);
+    const int all = ns_r32(K) / 32, t0 = all * group / KG, T = all * (group + 1) / KG - t0, most = (all + KG - 1) / KG;
+    qp += t0 * 128LL;
+    pp += t0 * 128LL;
+    const unsigned smem0 = mm_lds_addr(smem) + group * SLOTS * SLOT;
     constexpr int NI = decltype(lq)::NI;
     auto fetch = [&](bool rows, int step, int slot, auto piece) MM_INLINE {
         constexpr int k = decltype(piece)::value;
-        const long long at = (step < T ? step : T - 1) * 128LL;      // behind the last step it is fetched again, unused
+        const long long at = (step < T ? step : T > 0 ? T - 1 : -t0) * 128LL;      // behind the last step it is fetched again, unused
         const unsigned lds = smem0 + slot * SLOT + (k * C::WAVES + wave) * 1024;
         if (rows) mm_dma_s(lq.off[k], qp + at, lds);
         else mm_dma_s(lp.off[k], pp + at, lds);
@@ -199,7 +205,7 @@ __global__ __launch_bounds__(C::WAVES * 64) void ns_kernel(NsArgs a) {
     MmFrag<MM_KC, C::BN> fp;
     fq.init(lane, wm * C::TM);
     fp.init(lane, wn * C::TN);
-    mm_lds* const ring = (mm_lds*)smem;
+    mm_lds* const ring = (mm_lds*)smem + group * SLOTS * SLOT;
     s16x8 ph[2][NT], pl[2][NT], qh[MT], ql[MT];
     auto read_p = [&](mm_lds* slot, auto set, auto kf) MM_INLINE {
         constexpr int x = decltype(set)::value, f = decltype(kf)::value;
@@ -224,6 +230,7 @@ __global__ __launch_bounds__(C::WAVES * 64) void ns_kernel(NsArgs a) {
         constexpr int x = decltype(set)::value;
         mm_wait_dma<NI * (2 * D - 3)>();                              // stage t + 1 has landed, for everybody behind the barrier; stage t is read
         ga_lds_barrier();
+        if (KG > 1 && t >= T) return;                                 // another group has one step more
         const int nq = qs >= SLOTS - 2 ? qs + 2 - SLOTS : qs + 2, np = ps >= SLOTS - 2 ? ps + 2 - SLOTS : ps + 2;
         mm_for<0, MT>([&](auto ki) MM_INLINE {
             constexpr int i = decltype(ki)::value;
@@ -246,15 +253,33 @@ __global__ __launch_bounds__(C::WAVES * 64) void ns_kernel(NsArgs a) {
         qs = nq;
         ps = np;
     };
-    for (int t = 0; t < T; t += 2) {
+    for (int t = 0; t < most; t += 2) {
         step(t, std::integral_constant<int, 0>{});
-        if (t + 1 < T) step(t + 1, std::integral_constant<int, 1>{});
+        if (t + 1 < most) step(t + 1, std::integral_constant<int, 1>{});
     }
     mm_wait_dma<0>();
     ga_lds_barrier();
+    if constexpr (KG > 1) {
+        f32x4* sums = (f32x4*)smem;                                   // [group - 1][wave][tile][lane]
+        if (group > 0)
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) sums[(((group - 1) * C::WAVES + wave) * MT * NT + i * NT + j) * 64 + lane] = acc[i][j];
+        __syncthreads();
+        if (group == 0)
+#pragma unroll
+            for (int g = 1; g < KG; ++g)
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) acc[i][j] += sums[(((g - 1) * C::WAVES + wave) * MT * NT + i * NT + j) * 64 + lane];
+        __syncthreads();
+        if (group > 0) return;
+    }
 
-    // Epilogue, one 32 x 32 tile of a wave at a time: [m][n] with 8 consecutive n per lane, then [n][m] with 8 consecutive m.
-    float* st = (float*)smem + wave * (32 * 36);
+    // Epilogue, 32 rows x 16 columns of a wave at a time: [m][n] with 8 consecutive n per lane, then [n][m] with 8 consecutive m.
+    float* st = (float*)smem + wave * (32 * 20);
     char* XTn = a.flip ? mat.XT0 : mat.XT1;
     char* dst = KIND == NS_GRAM ? mat.A : KIND == NS_POLY ? mat.B : mat.X;
     const char* old = KIND == NS_POLY ? mat.A : mat.X;
@@ -263,18 +288,15 @@ __global__ __launch_bounds__(C::WAVES * 64) void ns_kernel(NsArgs a) {
 #pragma unroll
     for (int i = 0; i < MT / 2; ++i)
 #pragma unroll
-        for (int j = 0; j < NT / 2; ++j) {
+        for (int j = 0; j < NT; ++j) {
 #pragma unroll
-            for (int ii = 0; ii < 2; ++ii)
-#pragma unroll
-                for (int jj = 0; jj < 2; ++jj) *(f32x4*)(st + (16 * ii + (lane & 15)) * 36 + 16 * jj + 4 * (lane >> 4)) = acc[2 * i + ii][2 * j + jj];
+            for (int ii = 0; ii < 2; ++ii) *(f32x4*)(st + (16 * ii + (lane & 15)) * 20 + 4 * (lane >> 4)) = acc[2 * i + ii][j];
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            const int mb = m0 + wm * C::TM + 32 * i, nb = n0 + wn * C::TN + 32 * j;
-#pragma unroll
-            for (int p = 0; p < 2; ++p) {
-                const int row = p * 16 + (lane >> 2), c = (lane & 3) * 8, m = mb + row, n = nb + c;
+            const int mb = m0 + wm * C::TM + 32 * i, nb = n0 + wn * C::TN + 16 * j;
+            {
+                const int row = lane >> 1, c = (lane & 1) * 8, m = mb + row, n = nb + c;
                 float v[8];
-                mm_ldf8(st + row * 36 + c, v);
+                mm_ldf8(st + row * 20 + c, v);
                 if (m < M && n < ns_r32(N)) {
                     if (KIND == NS_GRAM) {
 #pragma unroll
@@ -298,24 +320,21 @@ __global__ __launch_bounds__(C::WAVES * 64) void ns_kernel(NsArgs a) {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) v[e] = 0.0f;          // rows beyond the last are columns of zeros of the transpose
                 }
-                mm_stf8(st + row * 36 + c, v);
+                mm_stf8(st + row * 20 + c, v);
             }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             if (KIND == NS_STEP ? (!user || mat.tall) : tm != tn) {
                 char* tr = KIND == NS_STEP ? XTn : dst;
+                const int mc = (lane >> 4) * 8, n = nb + (lane & 15), m = mb + mc;
+                float v[8];
 #pragma unroll
-                for (int p = 0; p < 2; ++p) {
-                    const int mc = p * 16 + (lane >> 5) * 8, n = nb + (lane & 31), m = mb + mc;
-                    float v[8];
+                for (int e = 0; e < 8; ++e) v[e] = st[(mc + e) * 20 + (lane & 15)];
+                if (n < N && m < ns_r32(M)) {
+                    if (!user) ns_put8(tr + n * ldm + ns_at(m), v);
+                    else {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] = st[(mc + e) * 36 + (lane & 31)];
-                    if (n < N && m < ns_r32(M)) {
-                        if (!user) ns_put8(tr + n * ldm + ns_at(m), v);
-                        else {
-#pragma unroll
-                            for (int e = 0; e < 8; ++e)
-                                if (m + e < M) ns_store<DT>(mat.o, n * mat.ldo + m + e, v[e] * (1.0f / NS_SCALE));
-                        }
+                        for (int e = 0; e < 8; ++e)
+                            if (m + e < M) ns_store<DT>(mat.o, n * mat.ldo + m + e, v[e] * (1.0f / NS_SCALE));
                     }
                 }
             }
@@ -326,8 +345,8 @@ __global__ __launch_bounds__(C::WAVES * 64) void ns_kernel(NsArgs a) {
 namespace {
 
 typedef MmGeom<64, 64, 4, 2> NsT;
-typedef MmGeom<128, 128, 4, 2> NsS;
-typedef MmGeom<192, 192, 4, 2> NsM;
+typedef MmGeom<128, 128, 8, 4> NsS;
+typedef MmGeom<192, 192, 8, 4> NsM;      // (two waves a SIMD: with one, more than 256 registers, and moves between their halves in the loop)
 
 size_t al(size_t n) { return (n + 255) & ~(size_t)255; }
 
@@ -352,17 +371,20 @@ template <class C> int ns_tiles(NsArgs& a, int kind) {
     return (int)at;
 }
 
-template <class C, int D, int KIND, int DT> int ns_go(NsArgs& a, hipStream_t st) {
+template <class C, int D, int KG, int KIND, int DT> int ns_go(NsArgs& a, hipStream_t st) {
     const int tiles = ns_tiles<C>(a, KIND);
-    hipLaunchKernelGGL((ns_kernel<C, D, KIND, DT>), dim3(tiles), dim3(C::WAVES * 64), 0, st, a);
+    hipLaunchKernelGGL((ns_kernel<C, D, KG, KIND, DT>), dim3(tiles), dim3(C::WAVES * KG * 64), 0, st, a);
     return hipGetLastError() == hipSuccess ? ACMIL_OK : ACMIL_ERR_LAUNCH;
 }
 
 template <int KIND, int DT> int ns_product(NsArgs& a, hipStream_t st) {
     // the largest tile that still gives most CUs work: larger tiles read less of LDS and L2 per flop
-    if (ns_tiles<NsM>(a, KIND) >= 200) return ns_go<NsM, 2, KIND, DT>(a, st);
-    if (ns_tiles<NsS>(a, KIND) >= 200) return ns_go<NsS, 2, KIND, DT>(a, st);
-    return ns_go<NsT, 4, KIND, DT>(a, st);
+    if (ns_tiles<NsM>(a, KIND) >= 200) return ns_go<NsM, 2, 1, KIND, DT>(a, st);
+    if (ns_tiles<NsS>(a, KIND) >= 200) return ns_go<NsS, 2, 1, KIND, DT>(a, st);
+    const int small = ns_tiles<NsT>(a, KIND);
+    if (small <= 256) return ns_go<NsT, 4, 2, KIND, DT>(a, st);       // one workgroup of two groups per CU, three steps ahead
+    if (small <= 512) return ns_go<NsT, 4, 1, KIND, DT>(a, st);       // two workgroups of one
+    return ns_go<NsT, 2, 1, KIND, DT>(a, st);
 }
 
 template <int DT> int ns_run(int count, const acmil_ortho_mat* mats, int steps, const float* co, float eps, char* ws, hipStream_t st) {
