@@ -10,7 +10,7 @@ enum { MM_KC = 0, MM_KS = 1 };   // operand element (row, k) lies at row * ld + 
 // MM_GATE_BWD: v = dh -> dg = dh u act'(g), du = dh act(g).  MM_PART: raw fp32 sums of one K range for mm_join.
 enum { MM_ACT = 0, MM_GATE = 1, MM_GATE_BWD = 2, MM_PART = 3 };
 
-enum { MM_S = 0, MM_L = 1, MM_D = 2 };   // tile configurations of mm16_kernel.h
+enum { MM_S = 0, MM_L = 1, MM_D = 2, MM_R32 = 3, MM_R64 = 4 };   // tile configurations of mm16_kernel.h
 
 struct MmEpi {
     int act, vec;                      // vec: every row that is touched starts on 16 bytes

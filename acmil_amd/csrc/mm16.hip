@@ -177,6 +177,19 @@ int mm_splits(long long tiles, int steps, double outputs) {
     return best;
 }
 
+// ... and of a product of up to 64 rows in 256-column tiles: a step streams 32 KB of P and the rows of Q, at 37 GB/s and CU (a workgroup
+// waits for memory alone) and at 5 TB/s altogether
+int slim_splits(long long tiles, int steps, int bm, double outputs) {
+    int best = 1;
+    double least = 1e30;
+    for (int s = 1; s <= 64 && s * 4 <= (steps > 4 ? steps : 4) && tiles * s <= 256; ++s) {
+        const double bytes = 128.0 * (256 + bm), all = (double)tiles * s * bytes / 5e6, one = bytes / 37e3;
+        const double us = ((steps + s - 1) / s) * (all > one ? all : one) + (s > 1 ? 2.5 + s * outputs * 8.0 / 4e6 : 0.0);
+        if (us < least) { least = us; best = s; }
+    }
+    return best;
+}
+
 // One product: tile, K split, launch, join.
 void product(Ctx& c, int kind, MmArgs a, int epi) {
     const bool dual = epi == MM_GATE;
@@ -185,18 +198,22 @@ void product(Ctx& c, int kind, MmArgs a, int epi) {
     // 256 x 256 tiles need half the LDS reads and fetches per flop of 128 x 128 ones, but only one fits a CU: taken where they fill
     // most of the 256 CUs
     const bool large = tl >= 160;
-    const int b = large ? 256 : 128;
-    a.ntm = (a.M + b - 1) / b;
-    a.ntn = (n_eff + b - 1) / b;
+    // up to 64 rows: tiles of as many rows where the weights have to be streamed (below 64 MB the 128-row tiles take 16 us for 64 x 4096 x 4096
+    // against 19, and 8.5 for 64 x 1024 x 1024 against 10.3)
+    const bool slim = !large && kind != WGRAD && a.M <= 64 && (double)n_eff * steps * 64 >= 33554432.0;
+    const int bm = large ? 256 : slim ? (a.M <= 32 ? 32 : 64) : 128, bn = large || slim ? 256 : 128;
+    a.ntm = (a.M + bm - 1) / bm;
+    a.ntn = (n_eff + bn - 1) / bn;
     const long long tiles = (long long)a.ntm * a.ntn;
-    a.splits = large ? 1 : mm_splits(tiles, steps, (double)a.M * r8(a.e.npad) * (dual ? 2 : 1));
+    const double outputs = (double)a.M * r8(a.e.npad) * (dual ? 2 : 1);
+    a.splits = large ? 1 : slim ? slim_splits(tiles, steps, bm, outputs) : mm_splits(tiles, steps, outputs);
     const size_t mark = c.ar.off;
     if (a.splits > 1) {
         a.e.ldpart = r8(a.e.npad);
         a.e.part = (float*)c.ar.take((size_t)a.splits * (dual ? 2 : 1) * a.M * a.e.ldpart * 4);
     }
     if (c.room() && c.go()) {
-        const int e = a.splits > 1 ? MM_PART : epi, cfg = large ? MM_L : tiles * a.splits <= 256 ? MM_D : MM_S;
+        const int e = a.splits > 1 ? MM_PART : epi, cfg = large ? MM_L : slim ? (bm == 32 ? MM_R32 : MM_R64) : tiles * a.splits <= 256 ? MM_D : MM_S;
         c.rc = kind == FWD ? mm_launch_fwd(a, c.bf, e, dual, cfg, c.st) : kind == DGRAD ? mm_launch_dgrad(a, c.bf, e, cfg, c.st)
                                                                              : mm_launch_wgrad(a, c.bf, e, cfg, c.st);
         if (a.splits > 1 && c.rc == ACMIL_OK) join(c, a, epi);
@@ -276,9 +293,18 @@ int linear_check(const acmil_linear_args* a, bool backward) {
     return ACMIL_OK;
 }
 
+bool plain(const Mat& m) { return on16(m.p) && m.ld % 8 == 0 && m.cols % 8 == 0; }
+
+// The kernel of mm16_rows.hip, or tiles of 32 rows?  The former reads x once per 16 to 64 columns beside the weights (3.1 TB/s at 24 rows
+// against 4.0), the latter takes two launches and rows on 16 bytes: worth it for 64 MB of weights and more (32 rows 4096 -> 4096: 15 us both).
+bool few_rows_wanted(const Mat& x, const Mat& w, int factors) {
+    if (x.rows > ACMIL_FEW_ROWS) return false;
+    return x.rows <= 4 || !plain(x) || !plain(w) || (double)factors * w.rows * w.cols < 33554432.0;
+}
+
 int linear_fwd(const acmil_linear_args& a, Ctx& c) {
     Mat x{a.x, a.ldx, a.M, a.K}, w{a.W, a.ldw, a.N, a.K};
-    const bool few = a.M <= ACMIL_FEW_ROWS;
+    const bool few = few_rows_wanted(x, w, 1);
     if (!few) { x = aligned(c, x); w = aligned(c, w); }
     MmArgs p = operands(x, w, a.M, a.N, x.cols, w.cols);
     output(p, a.y, a.ldy, a.bias, a.res, a.ldr);
@@ -338,9 +364,9 @@ int ffn_check(const acmil_ffn_args* a, bool backward) {
 
 int ffn_fwd(const acmil_ffn_args& a, Ctx& c) {
     const int F8 = r8(a.F);
-    const bool few = a.M <= ACMIL_FEW_ROWS;
     Mat x{a.x, a.ldx, a.M, a.D}, wg{a.Wg, a.ldwg, a.F, a.D}, wu{a.Wu, a.ldwu, a.F, a.D}, wd{a.Wd, a.ldwd, a.D, a.F};
-    if (!few) { x = aligned(c, x); aligned_pair(c, wg, wu); wd = aligned(c, wd); }
+    const bool few = few_rows_wanted(x, wg, 2) || (a.M <= ACMIL_FEW_ROWS && !plain(wu));
+    if (!few) { x = aligned(c, x); aligned_pair(c, wg, wu); }
     else if (wg.ld != wu.ld) aligned_pair(c, wg, wu);                // one leading dimension for both
     Mat h{a.h ? a.h : c.ar.take((size_t)a.M * F8 * 2), F8, a.M, F8};
     if (!c.room()) return c.rc;
@@ -351,9 +377,11 @@ int ffn_fwd(const acmil_ffn_args& a, Ctx& c) {
     p.e.bias2 = a.bu; p.e.npad = F8; p.e.act = a.act;
     p.e.pre = a.g; p.e.pre2 = a.u; p.e.ldp = F8;
     if (few) few_rows(c, p, true); else product(c, FWD, p, MM_GATE);
-    MmArgs d = operands(h, wd, a.M, a.D, few ? a.F : F8, few ? a.F : wd.cols);
+    const bool few_down = few_rows_wanted(h, wd, 1);
+    if (!few_down) wd = aligned(c, wd);
+    MmArgs d = operands(h, wd, a.M, a.D, few_down ? a.F : F8, few_down ? a.F : wd.cols);
     output(d, a.y, a.ldy, a.bd, a.res, a.ldr);
-    if (few) few_rows(c, d, false); else product(c, FWD, d, MM_ACT);
+    if (few_down) few_rows(c, d, false); else product(c, FWD, d, MM_ACT);
     return c.rc;
 }
 

@@ -39,11 +39,13 @@ template <int BM_, int BN_, int WAVES_, int WN_> struct MmGeom {
     static constexpr int QB = BM * 128, PB = BN * 128;
 };
 // MM_L: one 8-wave workgroup per CU.  MM_S: two 4-wave workgroups per CU.  MM_D: one 8-wave workgroup per CU that looks three steps ahead
-// instead of one -- alone on its CU a workgroup of MM_S waits a memory latency (about 1 us) for every second step.  D: steps of the ring, of
-// 2 D + 1 slots: all 160 KB of LDS or nearly.
+// instead of one -- alone on its CU a workgroup of MM_S waits a memory latency (about 1 us) for every second step.  MM_R32, MM_R64: few rows
+// by many columns, for products that are bound by streaming P.  D: steps of the ring, D + 1 slots of Q and D of P: 80 or up to 160 KB of LDS.
 template <int CFG> struct MmCfg;
 template <> struct MmCfg<MM_L> : MmGeom<256, 256, 8, 4> { static constexpr int D = 2, PER_SIMD = 2; };
 template <> struct MmCfg<MM_S> : MmGeom<128, 128, 4, 2> { static constexpr int D = 2, PER_SIMD = 2; };
+template <> struct MmCfg<MM_R32> : MmGeom<32, 256, 4, 4> { static constexpr int D = 4, PER_SIMD = 1; };
+template <> struct MmCfg<MM_R64> : MmGeom<64, 256, 4, 4> { static constexpr int D = 3, PER_SIMD = 1; };
 template <> struct MmCfg<MM_D> : MmGeom<128, 128, 8, 2> { static constexpr int D = 4, PER_SIMD = 2; };
 
 __device__ __forceinline__ unsigned mm_lds_addr(const void* p) { return (unsigned)(size_t)(const __attribute__((address_space(3))) void*)p; }
@@ -124,9 +126,9 @@ template <bool BF, int PK, int QK, int EPI, bool DUAL, int CFG>
 __global__ __launch_bounds__(MmCfg<CFG>::WAVES * 64, MmCfg<CFG>::PER_SIMD) void mm16_kernel(MmArgs a) {
     using C = MmCfg<CFG>;
     constexpr int MT = C::MT, NT = C::NT;
-    constexpr int SLOT = C::QB, D = C::D, SLOTS = 2 * D + 1;                           // half a stage: one operand of one K step
-    static_assert(C::QB == C::PB, "either operand fits any slot");
-    __shared__ __attribute__((aligned(128))) char smem[SLOTS * SLOT];
+    constexpr int D = C::D, RINGP = (D + 1) * C::QB;                 // D + 1 slots of Q, behind them D of P
+    __shared__ __attribute__((aligned(128))) char smem[RINGP + D * C::PB];
+    static_assert(C::WAVES * 32 * 68 * 4 <= RINGP + D * C::PB, "room for the turned tiles");
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / C::WN, wn = wave % C::WN;
 
@@ -165,7 +167,7 @@ __global__ __launch_bounds__(MmCfg<CFG>::WAVES * 64, MmCfg<CFG>::PER_SIMD) void 
 
     // Fetching one operand of one step in NI pieces.  Fetches are never skipped, so that their count is a constant: behind the last step
     // it is fetched again, unused.  TAIL (a K that is no multiple of 64): chunks beyond K come from the zero block.
-    constexpr int NI = decltype(lq)::NI;
+    constexpr int NIQ = decltype(lq)::NI, NIP = decltype(lp)::NI;
     struct Half { const char *from, *from2; unsigned lds; int k; };  // k: how much of K is left
     auto half_of = [&](int t, int slot, bool rows) MM_INLINE {
         t = t < t1 ? t : t1 - 1;
@@ -174,7 +176,7 @@ __global__ __launch_bounds__(MmCfg<CFG>::WAVES * 64, MmCfg<CFG>::PER_SIMD) void 
         Half h;
         h.from = rows ? (s1 ? a.q1 : a.q0) + qbase + tt * qstep : (s1 && !DUAL ? a.p1 : a.p0) + pbase + tt * pstep;
         h.from2 = DUAL && !rows ? a.p1 + pbase + tt * pstep : h.from;
-        h.lds = smem0 + slot * SLOT + wave * 1024;
+        h.lds = smem0 + (rows ? slot * C::QB : RINGP + slot * C::PB) + wave * 1024;
         h.k = (rows ? a.Kq : a.Kp) - tt * BK;
         return h;
     };
@@ -187,7 +189,7 @@ __global__ __launch_bounds__(MmCfg<CFG>::WAVES * 64, MmCfg<CFG>::PER_SIMD) void 
     auto fetch_p = [&](const Half& x, auto piece, auto tail) MM_INLINE {
         constexpr int i = decltype(piece)::value;
         const unsigned lds = x.lds + i * C::WAVES * 1024;
-        const char* from = DUAL && i >= NI / 2 ? x.from2 : x.from;
+        const char* from = DUAL && i >= NIP / 2 ? x.from2 : x.from;
         if constexpr (!decltype(tail)::value) mm_dma_s(lp.off[i], from, lds);
         else mm_dma_v(lp.k_of(i, wave, lane) < x.k ? from + lp.off[i] : (const char*)mm_zero, lds);
     };
@@ -203,11 +205,11 @@ __global__ __launch_bounds__(MmCfg<CFG>::WAVES * 64, MmCfg<CFG>::PER_SIMD) void 
     fq.init(lane, wm * C::TM);
     fp.init(lane, wn * (DUAL ? C::TN / 2 : C::TN));
 
-    // The ring has 2 D + 1 slots for Q_0 P_0 Q_1 P_1 Q_2 ...  A step is two pieces of 32 k.  A piece goes row tile by row tile: NT matrix
+    // The ring.  A step is two pieces of 32 k.  A piece goes row tile by row tile: NT matrix
     // instructions, then the row fragment just used is read again for the next piece (the column fragments, which every row tile needs,
     // have two register sets).  Between the pieces of step t a wave has read all it needs of Q_t and P_t, and its share of Q_(t+1) and
     // P_(t+1) has landed: behind the one barrier of the step the first fragments of step t + 1 are read.  Q_(t+D) is fetched during the
-    // first piece, into the slot that was free, and P_(t+D) during the second, into that of Q_t.  Fetches are spread over the step because
+    // first piece, into the slot of Q_(t-1), and P_(t+D) during the second, into that of P_t.  Fetches are spread over the step because
     // one that finds the address unit busy holds its wave up, with its matrix instructions: sent out in one burst behind the barrier
     // they cost 18 % more cycles.
     s16x8 p[2][NT], q[MT];
@@ -232,32 +234,29 @@ __global__ __launch_bounds__(MmCfg<CFG>::WAVES * 64, MmCfg<CFG>::PER_SIMD) void 
                 for (int j = 0; j < NT; ++j) acc[i][j] = mm_mfma<BF>(p[sub][j], q[i], acc[i][j]);
                 __builtin_amdgcn_sched_barrier(0);                   // else the read goes first, into registers that are not there
                 read_q(qslot, Other{}, ki);
-                mm_for<i * NI / MT, (i + 1) * NI / MT>([&](auto d) MM_INLINE {
-                    if constexpr (sub == 0) fetch_q(h, d, tail);
-                    else fetch_p(h, d, tail);
-                });
+                if constexpr (sub == 0) mm_for<i * NIQ / MT, (i + 1) * NIQ / MT>([&](auto d) MM_INLINE { fetch_q(h, d, tail); });
+                else mm_for<i * NIP / MT, (i + 1) * NIP / MT>([&](auto d) MM_INLINE { fetch_p(h, d, tail); });
                 __builtin_amdgcn_sched_barrier(0);
             });
         };
         mm_for<0, D>([&](auto i) MM_INLINE {
-            const Half hq = half_of(t0 + i, 2 * i, true), hp = half_of(t0 + i, 2 * i + 1, false);
-            mm_for<0, NI>([&](auto d) MM_INLINE { fetch_q(hq, d, tail); });
-            mm_for<0, NI>([&](auto d) MM_INLINE { fetch_p(hp, d, tail); });
+            const Half hq = half_of(t0 + i, i, true), hp = half_of(t0 + i, i, false);
+            mm_for<0, NIQ>([&](auto d) MM_INLINE { fetch_q(hq, d, tail); });
+            mm_for<0, NIP>([&](auto d) MM_INLINE { fetch_p(hp, d, tail); });
         });
-        mm_wait_dma<(2 * D - 2) * NI>();
+        mm_wait_dma<(D - 1) * (NIQ + NIP)>();
         ga_lds_barrier();
-        int qs = 0, ps = 1, free = SLOTS - 1;                        // slots of Q_t, P_t and the one that Q_(t+D) goes to
-        mm_for<0, NT>([&](auto f) MM_INLINE { read_p(ring + SLOT, std::integral_constant<int, 0>{}, f); });
+        int qs = 0, ps = 0;                                          // slots of Q_t and P_t
+        mm_for<0, NT>([&](auto f) MM_INLINE { read_p(ring + RINGP, std::integral_constant<int, 0>{}, f); });
         mm_for<0, MT>([&](auto f) MM_INLINE { read_q(ring, std::integral_constant<int, 0>{}, f); });
         for (int t = t0; t < t1; ++t) {
-            const Half hq = half_of(t + D, free, true), hp = half_of(t + D, qs, false);
-            piece(std::integral_constant<int, 0>{}, ring + qs * SLOT, ring + ps * SLOT, hq);
-            mm_wait_dma<(2 * D - 3) * NI>();                         // younger steps may still be on their way
+            const Half hq = half_of(t + D, qs == 0 ? D : qs - 1, true), hp = half_of(t + D, ps, false);
+            piece(std::integral_constant<int, 0>{}, ring + qs * C::QB, ring + RINGP + ps * C::PB, hq);
+            mm_wait_dma<(D - 1) * NIQ + (D - 2) * NIP>();            // younger steps may still be on their way
             ga_lds_barrier();
-            free = ps;
-            qs = qs >= SLOTS - 2 ? qs + 2 - SLOTS : qs + 2;
-            ps = ps >= SLOTS - 2 ? ps + 2 - SLOTS : ps + 2;
-            piece(std::integral_constant<int, 1>{}, ring + qs * SLOT, ring + ps * SLOT, hp);
+            qs = qs == D ? 0 : qs + 1;
+            ps = ps == D - 1 ? 0 : ps + 1;
+            piece(std::integral_constant<int, 1>{}, ring + qs * C::QB, ring + RINGP + ps * C::PB, hp);
         }
     };
     if (kmin == kmax && kmin % BK == 0) run(std::false_type{});
@@ -315,6 +314,10 @@ template <bool BF, int PK, int QK, int EPI, bool DUAL, int CFG> static inline in
 template <bool BF, int PK, int QK, int EPI, bool DUAL> static inline int mm_go_cfg(const MmArgs& a, int cfg, hipStream_t st) {
     // (K is never split where the large tiles fill the chip)
     if constexpr (EPI != MM_PART) if (cfg == MM_L) return mm_go<BF, PK, QK, EPI, DUAL, MM_L>(a, st);
+    if constexpr (QK == MM_KC) {                                      // few rows: not for weight gradients, whose rows are features
+        if (cfg == MM_R32) return mm_go<BF, PK, QK, EPI, DUAL, MM_R32>(a, st);
+        if (cfg == MM_R64) return mm_go<BF, PK, QK, EPI, DUAL, MM_R64>(a, st);
+    }
     return cfg == MM_D ? mm_go<BF, PK, QK, EPI, DUAL, MM_D>(a, st) : mm_go<BF, PK, QK, EPI, DUAL, MM_S>(a, st);
 }
 template <int PK, int QK, int EPI, bool DUAL> static inline int mm_go_any(const MmArgs& a, bool bf, int cfg, hipStream_t st) {

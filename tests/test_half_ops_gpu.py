@@ -66,6 +66,19 @@ def test_linear_large_tiles_and_split_products(M, K, N, dt):
     check_linear(x, w, b, "silu", r, dy)
 
 
+@pytest.mark.parametrize("M, K, N", [(5, 8200, 4100), (20, 4096, 8201), (32, 4104, 8208), (33, 8200, 4104), (64, 4096, 8200)])
+@pytest.mark.parametrize("dt", list(DTS))
+def test_few_rows_by_streamed_weights(M, K, N, dt):
+    """weights of 64 MB and more under 5 to 64 rows have tiles of their own (forward and input gradient)"""
+    x, w, b, r, dy = make_linear(M, K, N, DTS[dt], seed=M)
+    check_linear(x, w, b, "gelu_tanh", r, dy)
+
+
+@pytest.mark.parametrize("M", [24, 50])
+def test_ffn_few_rows_by_streamed_weights(M):
+    check_ffn(make_ffn(M, 4096, 8200, torch.bfloat16, seed=M), "silu")
+
+
 @pytest.mark.parametrize("M", [9, 90])
 def test_linear_strides(M):
     """row strides, shifted bases, transposed weights, expanded rows, leading dimensions, strided bias and residual"""
