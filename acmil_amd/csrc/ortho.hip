@@ -57,30 +57,49 @@ template <int DT> __device__ __forceinline__ void ns_store(void* p, long long i,
     else ((__bf16*)p)[i] = (__bf16)v;
 }
 
+// eight neighbouring values of a row, from column c (a multiple of 8); zeros at and beyond cols.  vec: rows start on 16 bytes
+template <int DT> __device__ __forceinline__ void ns_load8(const void* p, long long row, int c, int cols, bool vec, float* v) {
+    if (vec && c + 8 <= cols) {
+        if constexpr (DT == ACMIL_DTYPE_F32) mm_ldf8((const float*)p + row + c, v);
+        else mm_ld8<DT == ACMIL_DTYPE_BF16>(p, row + c, v);
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = c + j < cols ? ns_load<DT>(p, row + c + j) : 0.0f;
+}
+template <int DT> __device__ __forceinline__ bool ns_on16(const NsMat& m) {
+    return ((size_t)m.g & 15) == 0 && m.ldg % (DT == ACMIL_DTYPE_F32 ? 4 : 8) == 0;
+}
+
 // sum of squares, in 64 bits (a gradient's squares leave the range of 32): NS_PARTS partial sums per matrix, fixed order
-#define NS_PARTS 512
+#define NS_PARTS 256
 template <int DT> __global__ __launch_bounds__(256) void ns_norm_kernel(NsArgs a, double* part) {
     const NsMat& m = a.m[blockIdx.y];
-    const int rows = m.tall ? m.t : m.s, cols = m.tall ? m.s : m.t;
+    const int rows = m.tall ? m.t : m.s, cols = m.tall ? m.s : m.t, cpr = (cols + 7) / 8;
+    const bool vec = ns_on16<DT>(m);
+    const long long total = (long long)rows * cpr, step = NS_PARTS * 256LL;
     double s = 0.0;
-    // a row per quarter of the workgroup: 64 lanes x 4 neighbouring values
-    const int lane = threadIdx.x & 63;
-    for (int r = blockIdx.x * 4 + (threadIdx.x >> 6); r < rows; r += NS_PARTS * 4)
-        for (int c = lane * 4; c < cols; c += 256) {
-            float v[4];
+    for (long long i = blockIdx.x * 256LL + threadIdx.x; i < total; i += 2 * step) {
+        float v[2][8];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = c + j < cols ? ns_load<DT>(m.g, r * m.ldg + c + j) : 0.0f;
+        for (int h = 0; h < 2; ++h) {                                 // two chunks on their way at a time
+            const long long k = i + h * step, r = k / cpr;
+            if (k < total) ns_load8<DT>(m.g, r * m.ldg, (int)(k - r * cpr) * 8, cols, vec, v[h]);
+            else
 #pragma unroll
-            for (int j = 0; j < 4; ++j) s += (double)v[j] * (double)v[j];
+                for (int j = 0; j < 8; ++j) v[h][j] = 0.0f;
         }
-    __shared__ double red[256];
-    red[threadIdx.x] = s;
-    __syncthreads();
-    for (int o = 128; o > 0; o >>= 1) {
-        if ((int)threadIdx.x < o) red[threadIdx.x] += red[threadIdx.x + o];
-        __syncthreads();
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) s += (double)v[h][j] * (double)v[h][j];
     }
-    if (threadIdx.x == 0) part[blockIdx.y * NS_PARTS + blockIdx.x] = red[0];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+    __shared__ double red[4];
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) part[blockIdx.y * NS_PARTS + blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
 __device__ __forceinline__ void ns_put8(char* hi, const float* v) {          // eight scaled values -> their hi and lo halves
@@ -104,17 +123,28 @@ template <int DT> __global__ __launch_bounds__(256) void ns_split_kernel(NsArgs 
     const NsMat& m = a.m[mi];
     const int rows = m.tall ? m.t : m.s, cols = m.tall ? m.s : m.t;
     const int ct = (cols + 63) / 64, id = blockIdx.x - a.first[mi], r0 = id / ct * 64, c0 = id % ct * 64;
+    float in[2][8];
+    const bool vec = ns_on16<DT>(m);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int r = r0 + (threadIdx.x >> 3) + 32 * h, c = c0 + (threadIdx.x & 7) * 8;
+        if (r < rows) ns_load8<DT>(m.g, r * m.ldg, c, cols, vec, in[h]);
+        else
+#pragma unroll
+            for (int j = 0; j < 8; ++j) in[h][j] = 0.0f;
+    }
     if (threadIdx.x < 64) {                                           // every workgroup adds the partial sums up for itself, in one order
         double s = 0.0;
-        for (int i = threadIdx.x; i < NS_PARTS; i += 64) s += a.part[mi * NS_PARTS + i];
+#pragma unroll
+        for (int i = 0; i < NS_PARTS / 64; ++i) s += a.part[mi * NS_PARTS + i * 64 + threadIdx.x];
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
         if (threadIdx.x == 0) scale_s = (float)((double)NS_SCALE / (sqrt(s) + (double)a.eps));
     }
-    for (int i = threadIdx.x; i < 64 * 64; i += 256) {
-        const int r = r0 + (i >> 6), c = c0 + (i & 63);
-        tile[i >> 6][i & 63] = r < rows && c < cols ? ns_load<DT>(m.g, r * m.ldg + c) : 0.0f;
-    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) tile[(threadIdx.x >> 3) + 32 * h][(threadIdx.x & 7) * 8 + j] = in[h][j];
     __syncthreads();
     const float scale = scale_s;
     char* direct = m.tall ? m.XT0 : m.X;      // [rows][cols]
