@@ -118,7 +118,7 @@ __device__ __forceinline__ void ns_get8(const char* hi, float* v) {
 // G / (|G|_F + eps) in both orientations, 64 x 64 values per workgroup turned through LDS
 template <int DT> __global__ __launch_bounds__(256) void ns_split_kernel(NsArgs a) {
     __shared__ float tile[64][65];
-    __shared__ float scale_s;
+    __shared__ double scale_s;                                        // in 64 bits: 1 / |G| may leave the range of 32
     const int mi = ns_find(a, blockIdx.x);
     const NsMat& m = a.m[mi];
     const int rows = m.tall ? m.t : m.s, cols = m.tall ? m.s : m.t;
@@ -139,14 +139,15 @@ template <int DT> __global__ __launch_bounds__(256) void ns_split_kernel(NsArgs 
         for (int i = 0; i < NS_PARTS / 64; ++i) s += a.part[mi * NS_PARTS + i * 64 + threadIdx.x];
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
-        if (threadIdx.x == 0) scale_s = (float)((double)NS_SCALE / (sqrt(s) + (double)a.eps));
+        if (threadIdx.x == 0) scale_s = (double)NS_SCALE / (sqrt(s) + (double)a.eps);
     }
+    __syncthreads();
+    const double scale = scale_s;
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) tile[(threadIdx.x >> 3) + 32 * h][(threadIdx.x & 7) * 8 + j] = in[h][j];
+        for (int j = 0; j < 8; ++j) tile[(threadIdx.x >> 3) + 32 * h][(threadIdx.x & 7) * 8 + j] = (float)((double)in[h][j] * scale);
     __syncthreads();
-    const float scale = scale_s;
     char* direct = m.tall ? m.XT0 : m.X;      // [rows][cols]
     char* turned = m.tall ? m.X : m.XT0;      // [cols][rows]
 #pragma unroll
@@ -155,12 +156,12 @@ template <int DT> __global__ __launch_bounds__(256) void ns_split_kernel(NsArgs 
         float v[8];
         if (r0 + r < rows && c0 + c < ns_r32(cols)) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = tile[r][c + j] * scale;
+            for (int j = 0; j < 8; ++j) v[j] = tile[r][c + j];
             ns_put8(direct + (r0 + r) * ns_ld(cols) + ns_at(c0 + c), v);
         }
         if (c0 + r < cols && r0 + c < ns_r32(rows)) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = tile[c + j][r] * scale;
+            for (int j = 0; j < 8; ++j) v[j] = tile[c + j][r];
             ns_put8(turned + (c0 + r) * ns_ld(rows) + ns_at(r0 + c), v);
         }
     }

@@ -85,7 +85,7 @@ def test_low_rank_zero_and_scale():
     check(o, g)
     assert not ops.orthogonalize(torch.zeros(70, 90, device="cuda")).any()
     g = gradient(96, 160, torch.float32, scale=1.0)
-    for s in (1e-30, 1e-4, 1e20, 1e30):                                                      # squares that leave fp32
+    for s in (1e-34, 1e-30, 1e-4, 1e20, 1e30):                                                # squares and reciprocals that leave fp32
         o = ops.orthogonalize(g * s, eps=0.0)
         assert (o - ops.orthogonalize(g, eps=0.0)).norm() <= 1e-4 * o.norm(), s              # scaling rounds every value by 2^-24, times at most 3.9^5
     g[3, 4] = float("inf")
