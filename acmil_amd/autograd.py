@@ -348,7 +348,10 @@ class _LinearAct(torch.autograd.Function):
 
 
 def linear_act(x, weight, bias=None, act="none", residual=None):
-    """Differentiable ops.linear_act: act(x @ weight^T + bias) + residual for fp16 / bf16 tensors (no double backward)."""
+    """Differentiable ops.linear_act: act(x @ weight^T + bias) + residual for fp16 / bf16 tensors (no double backward, no autocast: the
+    tensors are taken as they are)."""
+    if not torch.is_grad_enabled():
+        return ops.linear_act(x, weight, bias=bias, act=act, residual=residual)
     return _LinearAct.apply(x, weight, bias, residual, act)
 
 
@@ -378,5 +381,7 @@ class _GatedFfn(torch.autograd.Function):
 
 def gated_ffn(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None, act="silu", residual=None):
     """Differentiable ops.gated_ffn: (act(x @ w_gate^T + b_gate) * (x @ w_up^T + b_up)) @ w_down^T + b_down + residual for fp16 / bf16
-    tensors (no double backward)."""
+    tensors (no double backward, no autocast: the tensors are taken as they are)."""
+    if not torch.is_grad_enabled():
+        return ops.gated_ffn(x, w_gate, w_up, w_down, b_gate=b_gate, b_up=b_up, b_down=b_down, act=act, residual=residual)
     return _GatedFfn.apply(x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual, act)

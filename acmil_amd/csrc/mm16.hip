@@ -254,9 +254,10 @@ void colsum(Ctx& c, const Mat& x, int rows, int cols, void* out) {
     c.ar.off = mark;
 }
 
-// 32-bit byte offsets inside a tile: 256 rows (64 k rows) of the largest leading dimension; 31-bit row and column counts
+// 32-bit byte offsets inside a tile: 256 rows (64 k rows) of the largest leading dimension; 31-bit row, column and tile counts
 const long long MAX_LD = 1LL << 22;
-const int MAX_DIM = 1 << 22;
+const int MAX_DIM = 1 << 22, MAX_ROWS = 1 << 30;
+const double MAX_OUT = 274877906944.0;       // 2^38 outputs, more than the memory holds: at most 2^23 tiles, 2^32 threads
 
 bool same_dtype_ok(int dtype) { return dtype == ACMIL_DTYPE_F16 || dtype == ACMIL_DTYPE_BF16; }
 bool act_ok(int act) { return act >= ACMIL_ACT_NONE && act <= ACMIL_ACT_SIGMOID; }
@@ -279,7 +280,8 @@ void few_rows(Ctx& c, MmArgs a, bool dual) {
 int linear_check(const acmil_linear_args* a, bool backward) {
     if (!a) return ACMIL_ERR_NULL;
     if (!same_dtype_ok(a->dtype)) return ACMIL_ERR_UNSUPPORTED;
-    if (!act_ok(a->act) || a->M <= 0 || a->K <= 0 || a->N <= 0 || a->K > MAX_DIM || a->N > MAX_DIM) return ACMIL_ERR_SHAPE;
+    if (!act_ok(a->act) || a->M <= 0 || a->K <= 0 || a->N <= 0 || a->M > MAX_ROWS || a->K > MAX_DIM || a->N > MAX_DIM) return ACMIL_ERR_SHAPE;
+    if ((double)a->M * a->N > MAX_OUT || (double)a->M * a->K > MAX_OUT) return ACMIL_ERR_SHAPE;
     if (!a->x || !a->W) return ACMIL_ERR_NULL;
     if (!ld_ok(a->x, a->ldx, a->K) || !ld_ok(a->W, a->ldw, a->K)) return ACMIL_ERR_SHAPE;
     if (!backward) {
@@ -348,7 +350,8 @@ int linear_bwd(const acmil_linear_args& a, Ctx& c) {
 int ffn_check(const acmil_ffn_args* a, bool backward) {
     if (!a) return ACMIL_ERR_NULL;
     if (!same_dtype_ok(a->dtype)) return ACMIL_ERR_UNSUPPORTED;
-    if (!act_ok(a->act) || a->M <= 0 || a->D <= 0 || a->F <= 0 || a->D > MAX_DIM || a->F > MAX_DIM / 2) return ACMIL_ERR_SHAPE;
+    if (!act_ok(a->act) || a->M <= 0 || a->D <= 0 || a->F <= 0 || a->M > MAX_ROWS || a->D > MAX_DIM || a->F > MAX_DIM / 2) return ACMIL_ERR_SHAPE;
+    if ((double)a->M * a->D > MAX_OUT || (double)a->M * a->F > MAX_OUT / 2) return ACMIL_ERR_SHAPE;
     if (!a->x || !a->Wg || !a->Wu || !a->Wd) return ACMIL_ERR_NULL;
     if (!ld_ok(a->x, a->ldx, a->D) || !ld_ok(a->Wg, a->ldwg, a->D) || !ld_ok(a->Wu, a->ldwu, a->D) || !ld_ok(a->Wd, a->ldwd, a->F)) return ACMIL_ERR_SHAPE;
     const int saved = (a->g != nullptr) + (a->u != nullptr) + (a->h != nullptr);

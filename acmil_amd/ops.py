@@ -958,7 +958,7 @@ def linear_f16x3(x: torch.Tensor, packed: torch.Tensor, n_out: int, bias: Option
 # 16-bit linear layer with a fused epilogue, gated feed-forward block (csrc/mm16*.hip)
 # ---------------------------------------------------------------------------------------------------------------------
 _HALF = (torch.float16, torch.bfloat16)
-_MAX_ROWS, _MAX_DIM, _MAX_LD = (1 << 31) - 1, 1 << 22, 1 << 22
+_MAX_ROWS, _MAX_DIM, _MAX_LD = 1 << 30, 1 << 22, 1 << 22
 _NO_WORKSPACE_ROWS = 4     # acmil_linear_act of at most so many rows takes no workspace
 
 
@@ -1102,8 +1102,8 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     """acmil_gated_ffn: y = (act(x @ w_gate^T + b_gate) * (x @ w_up^T + b_up)) @ w_down^T + b_down + residual, fp16 or bf16, two launches:
     both projections, the activation and the product in one, the projection back with bias and residual in the other.  x [..., D], w_gate and
     w_up [F, D], w_down [D, F], residual [..., D]; act as linear_act ("silu" is the SwiGLU block, "gelu" GeGLU, "sigmoid" GLU, ...).
-    The gated features between the launches are held in x's type.  keep: also (g, u, h) for gated_ffn_bwd (g, u fp32 and h, each
-    [rows, round8(F)]).  No gradient is recorded (acmil_amd.autograd.gated_ffn is the differentiable form)."""
+    The gated features between the launches are held in x's type (in fp16, beyond 65504 they are infinite).  keep: also (g, u, h) for
+    gated_ffn_bwd (g, u fp32 and h, each [rows, round8(F)]).  No gradient is recorded (acmil_amd.autograd.gated_ffn is the differentiable form)."""
     dev = _half_inputs("gated_ffn", x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual)
     a, hold = _ffn_args("gated_ffn", x, w_gate, w_up, w_down, act)
     bg, bu, bd = _vec16("gated_ffn", "b_gate", b_gate, a.F), _vec16("gated_ffn", "b_up", b_up, a.F), _vec16("gated_ffn", "b_down", b_down, a.D)

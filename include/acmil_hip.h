@@ -614,7 +614,7 @@ int acmil_adamw_step_peer(float* params, float* exp_avg, float* exp_avg_sq, long
  * workspace: acmil_*_workspace_bytes(args) bytes, 256-byte aligned, contents arbitrary, dead when the call's work is done.  The
  * query reads the same argument block (base addresses included: they decide about copies); 0 = the arguments are refused.
  * acmil_linear_act of at most 4 rows needs no workspace (NULL).
- * 1 <= M; 1 <= K, N, D <= 2^22, F <= 2^21; leading dimensions <= 2^22.
+ * 1 <= M <= 2^30; 1 <= K, N, D <= 2^22, F <= 2^21; leading dimensions <= 2^22; at most 2^38 outputs.  Outputs must not overlap inputs.
  * ------------------------------------------------------------------------------------------- */
 #define ACMIL_FEW_ROWS 32     /* acmil_linear_act and acmil_gated_ffn of at most so many rows read the weights straight from memory */
 #define ACMIL_ACT_NONE 0
@@ -668,7 +668,7 @@ int acmil_gated_ffn_bwd(const acmil_ffn_args* args, void* workspace, size_t work
  * dimensions ldg, ldo >= n (elements); o may be g.  1 <= m, n <= 65536.  coeffs: HOST array [steps][3], 1 <= steps <= 64; refused
  * (ACMIL_ERR_SHAPE) unless the polynomials keep singular values that start in [0, 1] below 3.9 and |b s^2 + c s^4| below 15.5.
  * Values are held as f16 pairs (22 bits) and products accumulate in fp32, whatever the type of g; the norm is formed in 64 bits.
- * A zero matrix gives zeros; infinities or NaN in g give NaN.  Reproducible bit for bit.
+ * A zero matrix gives zeros (eps > 0); infinities or NaN in g give NaN.  Reproducible bit for bit.
  * workspace: acmil_orthogonalize_workspace_bytes(...) (0 = refused), 256-byte aligned, contents arbitrary.
  * ------------------------------------------------------------------------------------------- */
 typedef struct acmil_ortho_mat {

@@ -18,6 +18,7 @@ def test_cpu_tensors_and_other_types_are_refused():
 
 @pytest.mark.parametrize("change, code", [
     ({}, -3), ({"dtype": 0}, -2), ({"dtype": 7}, -2), ({"act": 9}, -1), ({"M": 0}, -1), ({"K": 0}, -1), ({"N": -1}, -1), ({"K": (1 << 22) + 1}, -1),
+    ({"M": (1 << 30) + 1}, -1), ({"M": 1 << 30, "N": 1 << 12}, -1),
     ({"x": 4096, "W": 4096, "ldx": 15, "ldw": 16}, -1), ({"x": 4096, "W": 4096, "ldx": 16, "ldw": 1 << 23}, -1), ({"x": 4096, "W": 4096, "ldx": 16, "ldw": 16}, -3),
     ({"x": 4096, "W": 4096, "ldx": 16, "ldw": 16, "y": 4096, "ldy": 7}, -1),
     ({"x": 4096, "W": 4096, "ldx": 16, "ldw": 16, "y": 4096, "ldy": 8, "pre": 4100}, -1),

@@ -254,6 +254,41 @@ def test_refusals_on_the_device():
         torch.autograd.grad(gx.sum(), x)
 
 
+def test_without_gradients_nothing_is_kept():
+    x, w, b, r, dy = make_linear(70, 64, 40, torch.bfloat16)
+    t = make_ffn(70, 64, 40, torch.bfloat16)
+    w.requires_grad_(), t["wg"].requires_grad_()
+    with torch.no_grad():
+        y = autograd.linear_act(x, w, bias=b, act="silu", residual=r)
+        z = autograd.gated_ffn(t["x"], t["wg"], t["wu"], t["wd"])
+    assert not y.requires_grad and not z.requires_grad
+    assert torch.equal(y, autograd.linear_act(x, w, bias=b, act="silu", residual=r)) and torch.equal(z, autograd.gated_ffn(t["x"], t["wg"], t["wu"], t["wd"]))
+
+
+def test_gradients_against_differences():
+    """a directional derivative of the whole block against a central difference in 64 bits of the formulas: the gradients are off by at most their
+    bounds (half_reference), summed along the direction"""
+    t = make_ffn(40, 24, 32, torch.float16, seed=3)
+    names = ("x", "wg", "wu", "wd", "bg", "bu", "bd")
+    for k in names:
+        t[k].requires_grad_()
+    y = autograd.gated_ffn(*(t[k] for k in names), act="gelu_tanh", residual=t["r"])
+    got = torch.autograd.grad(y, [t[k] for k in names], t["dy"])
+    ref = R.ffn_ref(*(t[k] for k in names), "gelu_tanh", t["r"], t["dy"])
+    v = {k: t[k].detach().double() for k in names}
+
+    def value(p):
+        g, u = p["x"] @ p["wg"].t() + p["bg"], p["x"] @ p["wu"].t() + p["bu"]
+        return (((R.act64("gelu_tanh", g)[0] * u) @ p["wd"].t() + p["bd"]) * t["dy"].double()).sum()
+
+    for k, d in zip(names, got):
+        e = torch.randn(v[k].shape, generator=torch.Generator(device="cuda").manual_seed(7), device="cuda", dtype=torch.float64)
+        h = 1e-5
+        slope = (value({**v, k: v[k] + h * e}) - value({**v, k: v[k] - h * e})) / (2 * h)
+        bound = (ref["d" + k].off * e.abs()).sum() + 1e-6 * (1 + slope.abs())
+        assert (slope - (d.double() * e).sum()).abs() <= bound, k
+
+
 def test_mixed_needs():
     """only the gradients that are asked for are formed; the others are None"""
     x, w, b, r, dy = make_linear(50, 64, 40, torch.bfloat16)
