@@ -16,6 +16,10 @@ copies (cat / pad / slicing / `+`) and the dropout mask.  CUDA fp32 tensors only
   attn_pool(h, A)                softmax over N, then P @ h           -> softmax_rows + matmul
   linear_act(x, W, b, act, r)    16-bit act(x W^T + b) + r            -> acmil_linear_act/_bwd   (fp16 / bf16 tensors)
   gated_ffn(x, Wg, Wu, Wd, ...)  16-bit gated feed-forward block      -> acmil_gated_ffn/_bwd    (fp16 / bf16 tensors)
+
+Graph captures: forward calls and the explicit backward forms (ops.linear_act_bwd, ops.gated_ffn_bwd) can be captured as they are.  A
+`backward()` of these Functions inside a capture must find no earlier autograd graph of the same leaves alive: torch accumulates into a
+leaf on the stream of its first graph, and that stream is not part of the capture.
 """
 from __future__ import annotations
 

@@ -1157,6 +1157,25 @@ def gated_ffn_bwd(dy: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w_up:
             None if bgu is None else bgu[:F], None if bgu is None else bgu[f8:f8 + F], bd)
 
 
+def _no_overlap(gs, outs) -> None:
+    """Nothing is written that another matrix of an orthogonalize call reads or writes; g[i] and out[i] may be the same memory."""
+    spans = []
+    for i, (g, o) in enumerate(zip(gs, outs)):
+        if g.numel():
+            end = 1 + sum((n - 1) * s for n, s in zip(g.shape, g.stride()))
+            own = (g.data_ptr(), g.data_ptr() + end * g.element_size())
+            to = (o.data_ptr(), o.data_ptr() + o.numel() * o.element_size())
+            if own != to or not g.is_contiguous():
+                spans.append(own + (False,))
+            spans.append(to + (True,))
+    reach = written = 0                                            # ends of what lies in front: of everything, of the outputs
+    for start, end, write in sorted(spans):
+        if start < (reach if write else written):
+            raise RuntimeError("acmil_amd.orthogonalize: out overlaps another matrix of the call")
+        reach = max(reach, end)
+        written = max(written, end if write else 0)
+
+
 NS_COEFFS = (3.4445, -4.7750, 2.0315)      # drives singular values from [0.002, 1] into [0.68, 1.14] in 5 steps
 
 
@@ -1165,7 +1184,7 @@ def orthogonalize(g, steps: int = 5, coeffs: Sequence = NS_COEFFS, eps: float = 
     then `steps` times X <- a X + (b A + c A A) X with A = X X^T, on the transpose where a matrix is tall.
     g: [m, n], a stack [..., m, n], or a list of [m, n] of any shapes (one type and device): all matrices share the launches.  fp32, fp16 or bf16,
     returned in the same type and structure; values are held to 22 bits inside whatever the type.  coeffs: one (a, b, c) or one per step.
-    out: contiguous tensor(s) of g's structure, type and shapes to write to; g itself will do."""
+    out: contiguous tensor(s) of g's structure, type and shapes to write to; a matrix may be its own output, other overlaps are refused."""
     lib = _lib.load()
     many = isinstance(g, (list, tuple))
     ts = list(g) if many else [g]
@@ -1184,6 +1203,8 @@ def orthogonalize(g, steps: int = 5, coeffs: Sequence = NS_COEFFS, eps: float = 
     if out is not None and (len(outs) != len(ts) or any(o.shape != t.shape or o.dtype != dt or o.device != dev or not o.is_contiguous()
                                                        for o, t in zip(outs, ts))):
         raise RuntimeError("acmil_amd.orthogonalize: out must be contiguous tensors of g's structure, type and shapes")
+    if out is not None:
+        _no_overlap(ts, outs)
     mats, hold = [], []
     for t, o in zip(ts, outs):
         if t.numel() == 0:

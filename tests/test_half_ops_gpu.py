@@ -237,6 +237,80 @@ def test_two_graphs_share_nothing():
         assert torch.equal(y1, e1) and torch.equal(y2, e2)
 
 
+def test_two_calls_at_once():
+    """two streams in turn, without waiting for each other: every call has a workspace of its own"""
+    lin = [make_linear(200, 1024, 320, torch.bfloat16, seed=k) for k in (0, 1)]
+    ffn = [make_ffn(200, 256, 320, torch.bfloat16, seed=k) for k in (0, 1)]
+
+    def step(k):
+        x, w, b, r, dy = lin[k]
+        t = ffn[k]
+        y, saved = ops.gated_ffn(t["x"], t["wg"], t["wu"], t["wd"], keep=True)
+        return (ops.linear_act(x, w, bias=b, act="silu", residual=r), y) + ops.linear_act_bwd(dy, x, w) + ops.gated_ffn_bwd(
+            t["dy"], t["x"], t["wg"], t["wu"], t["wd"], saved)[:4]
+
+    want = [step(0), step(1)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for k in (0, 1):
+            with torch.cuda.stream(streams[k]):
+                got[k].append(step(k))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for k in (0, 1) for out in got[k] for a, b in zip(out, want[k]))
+
+
+def test_one_tensor_in_two_places():
+    """the weight is also the input (its gradients add up, in the tensors' type), the residual is the input, one matrix is gate and up"""
+    w, dy = make_linear(96, 96, 96, torch.bfloat16)[1].detach(), make_linear(96, 96, 96, torch.bfloat16)[4]
+    w.requires_grad_()
+    (got,) = torch.autograd.grad(autograd.linear_act(w, w, act="silu", residual=w), w, dy)
+    parts = [w.detach().clone().requires_grad_() for _ in range(3)]
+    dx, dw, dr = torch.autograd.grad(autograd.linear_act(parts[0], parts[1], act="silu", residual=parts[2]), parts, dy)
+    exact = dx.double() + dw.double() + dr.double()                                          # two roundings of partial sums, in any order
+    assert ((got.double() - exact).abs() <= 2.0 ** -8 * (2.01 * (dx.abs() + dw.abs() + dr.abs()).double())).all()
+    t = make_ffn(50, 64, 40, torch.float16)
+    t["wu"] = t["wg"]
+    x, wg, wd = (t[k].requires_grad_() for k in ("x", "wg", "wd"))
+    (got,) = torch.autograd.grad(autograd.gated_ffn(x, wg, wg, wd), wg, t["dy"])
+    wu = wg.detach().clone().requires_grad_()
+    dg, du = torch.autograd.grad(autograd.gated_ffn(x, wg, wu, wd), (wg, wu), t["dy"])
+    assert torch.equal(got, dg + du)
+
+
+def test_offsets_beyond_32_bits():
+    """Inputs, outputs and kept values of more than 2^31 elements.  Only the last rows of dy are not zero: the weight gradients are exactly those of
+    these rows (zeros add nothing to a sum), and the values of these rows those of a small call."""
+    M, K, N, last = 270001, 8192, 16, 150
+    g = torch.Generator(device="cuda").manual_seed(9)
+    dt = torch.bfloat16
+    x = torch.zeros(M, K, dtype=dt, device="cuda")
+    dy = torch.zeros(M, N, dtype=dt, device="cuda")
+    x[-last:], dy[-last:] = rand(g, dt, last, K), rand(g, dt, last, N)
+    w, b = rand(g, dt, N, K, scale=K ** -0.5), rand(g, dt, N)
+    y, pre = ops.linear_act(x, w, bias=b, act="silu", keep_pre=True)
+    dx, dw, db = ops.linear_act_bwd(dy, x, w, pre, act="silu")
+    ref = R.linear_ref(x[-last:], w, b, "silu", None, dy[-last:])
+    for name, v in (("y", y[-last:]), ("dx", dx[-last:]), ("dw", dw), ("db", db)):
+        R.check(name, v, ref[name])
+    assert not dx[:-last].any()
+    del dx, pre, y
+    y = ops.linear_act(x[:, :N], w[:, :N].repeat(K // N, 1), act="relu")                    # the output is the large one
+    R.check("y", y[-last:], R.linear_ref(x[-last:, :N], w[:, :N].repeat(K // N, 1), None, "relu", None)["y"])
+    assert not y[:-last].any()
+    del x, y
+    t = make_ffn(1, N, K, dt, seed=4)
+    xs = torch.zeros(M, N, dtype=dt, device="cuda")
+    xs[-last:] = rand(g, dt, last, N)
+    y, saved = ops.gated_ffn(xs, t["wg"], t["wu"], t["wd"], keep=True)
+    dx, dg, du, dd = ops.gated_ffn_bwd(dy, xs, t["wg"], t["wu"], t["wd"], saved)[:4]
+    ref = R.ffn_ref(xs[-last:], t["wg"], t["wu"], t["wd"], None, None, None, "silu", None, dy[-last:])
+    for name, v in (("y", y[-last:]), ("dx", dx[-last:]), ("dwg", dg), ("dwu", du), ("dwd", dd)):
+        R.check(name, v, ref[name])
+    assert not dx[:-last].any() and not y[:-last].any()
+
+
 def test_refusals_on_the_device():
     x, w, b, r, dy = make_linear(4, 16, 8, torch.float16)
     bad = [lambda: ops.linear_act(x.float(), w), lambda: ops.linear_act(x, w.bfloat16()), lambda: ops.linear_act(x[:, :8], w),

@@ -125,6 +125,27 @@ def test_stream_graph_and_repeatability():
         assert all(torch.equal(a, b) for a, b in zip(want, held))
 
 
+def test_outputs_given_by_the_caller():
+    gs = [gradient(40, 64, torch.float32, seed=k) for k in range(30)]                        # two groups: the second is read when the first is written
+    want = ops.orthogonalize(gs)
+    outs = [torch.full((40, 64), 7.0, device="cuda") for _ in gs]
+    assert ops.orthogonalize(gs, out=outs)[3] is outs[3] and all(torch.equal(a, b) for a, b in zip(want, outs))
+    wide = torch.full((40, 80), 7.0, device="cuda")                                          # between rows that are not its own nothing is written
+    wide[:, 8:72] = gs[0]
+    assert torch.equal(ops.orthogonalize(wide[:, 8:72], out=outs[0]), want[0]) and (wide[:, :8] == 7).all() and (wide[:, 72:] == 7).all()
+    buf = torch.stack(gs)
+    for out in (torch.empty(30, 64, 40, device="cuda"), torch.empty(30, 64, 40, device="cuda").transpose(1, 2), outs[0], torch.empty_like(buf).half()):
+        with pytest.raises(RuntimeError, match="structure"):
+            ops.orthogonalize(buf, out=out)
+    for a, out in ((gs, gs[1:] + gs[:1]), (gs, [outs[0]] * 30), ([buf[0], buf[1]], [buf.view(-1)[640:3200].view(40, 64), outs[1]]),
+                   (wide[:, 8:72], wide.view(-1)[:2560].view(40, 64))):
+        with pytest.raises(RuntimeError, match="overlaps"):
+            ops.orthogonalize(a, out=out)
+    assert ops.orthogonalize([gs[0], gs[0]])[1].equal(want[0])                               # read twice: allowed
+    ops.orthogonalize(buf, out=buf), ops.orthogonalize(gs, out=gs)
+    assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(want, gs, buf))
+
+
 def test_refusals():
     g = gradient(8, 8, torch.float32)
     for call in (lambda: ops.orthogonalize(g.double()), lambda: ops.orthogonalize(g[0]), lambda: ops.orthogonalize([g, g.half()]),
