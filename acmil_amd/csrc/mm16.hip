@@ -4,69 +4,81 @@
 #include "mm16.h"
 
 // ------------------------------------------------------------------------------------------------ small kernels
-// src [rows, cols] (any leading dimension, any alignment of 2 bytes) -> dst [rows, ldd], ldd = round8(cols), zero-filled: the one
-// shape whose rows the LDS-DMA can fetch in 16-byte chunks.  Only matrices that are not already so pass through here.
-__global__ __launch_bounds__(256) void mm_pad_kernel(const short* __restrict__ src, long long lds, int rows, int cols, short* __restrict__ dst, int ldd) {
-    const int cpr = ldd / 8;
-    const long long total = (long long)rows * cpr;
-    for (long long i = blockIdx.x * 256LL + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
-        const int r = (int)(i / cpr), c = (int)(i - (long long)r * cpr) * 8;
-        const short* s = src + r * lds + c;
+// Up to MM_PADS matrices src [rows, cols] (any leading dimension, any alignment of 2 bytes) -> dst [rows, ldd], ldd = round8(cols),
+// zero-filled: the one shape whose rows the LDS-DMA can fetch in 16-byte chunks.  Only matrices that are not already so pass through here, all
+// of a call in one launch: a training step of odd sizes is bound by its launches.
+#define MM_PADS 5
+struct MmPads {
+    int count;
+    struct { const short* src; short* dst; long long lds, first; int rows, cols, ldd; } m[MM_PADS];     // first: chunks of the matrices in front
+    long long total;
+};
+__global__ __launch_bounds__(256) void mm_pad_kernel(MmPads a) {
+    for (long long i = blockIdx.x * 256LL + threadIdx.x; i < a.total; i += (long long)gridDim.x * 256) {
+        int k = 0;
+#pragma unroll
+        for (int j = 1; j < MM_PADS; ++j) k += j < a.count && i >= a.m[j].first;
+        const int cols = a.m[k].cols, ldd = a.m[k].ldd, cpr = ldd / 8;
+        const long long q = i - a.m[k].first;
+        const int r = (int)(q / cpr), c = (int)(q - (long long)r * cpr) * 8;
+        const short* s = a.m[k].src + r * a.m[k].lds + c;
         short v[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = c + j < cols ? s[j] : (short)0;
-        *(uint4*)(dst + (long long)r * ldd + c) = *(const uint4*)v;
+        *(uint4*)(a.m[k].dst + (long long)r * ldd + c) = *(const uint4*)v;
     }
 }
 
-// dz = dy act'(z), z kept in fp32; columns N .. ldz - 1 become zero
-template <bool BF>
-__global__ __launch_bounds__(256) void mm_dz_kernel(const void* __restrict__ dy, long long lddy, int vec, const float* __restrict__ z, long long ldp, int act,
-                                                    int M, int N, void* __restrict__ dz, int ldz) {
-    const int cpr = ldz / 8;
-    const long long total = (long long)M * cpr;
-    for (long long i = blockIdx.x * 256LL + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
-        const int m = (int)(i / cpr), n = (int)(i - (long long)m * cpr) * 8;
-        float d[8], p[8];
-        mm_row8<BF>(dy, m * lddy, n, N, vec != 0, d);
-        mm_ldf8(z + m * ldp + n, p);
-        float a[8], slope[8];
-        mm_act_slope8(act, p, a, slope);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) d[j] *= slope[j];
-        mm_put8<BF>(dz, (long long)m * ldz, n, N, ldz, true, d);
-    }
-}
-
-// Column sums in two passes of fixed order: a workgroup adds its rows of 256 columns (8 row lanes x 32 chunks), part [gy][ldc] holds
-// what the second pass adds up.
-template <bool BF>
-__global__ __launch_bounds__(256) void mm_colsum_kernel(const void* __restrict__ x, long long ld, int rows, int cols8, float* __restrict__ part) {
-    __shared__ float red[8][32][9];
-    const int cx = threadIdx.x & 31, ry = threadIdx.x >> 5, c = (blockIdx.x * 32 + cx) * 8;
+// Column sums, and dz on the way.  DZ: dz = dy act'(z) with z kept in fp32, stored as [rows][cols8] with zeros behind column cols - 1, and the
+// sums (if wanted) are those of its values before they are rounded; else: x [rows][cols8] as it lies.  A workgroup takes a run of rows of
+// 8 << lcx columns, 256 >> lcx rows a time.  Sums go to part [gridDim.y][cols8], or straight to out where one workgroup has all rows: two
+// passes of fixed order, no atomics.  Bound by its bytes: 8 a value with dz, 2 without.
+template <bool BF, bool DZ>
+__global__ __launch_bounds__(256) void mm_colsum_kernel(const void* __restrict__ x, long long ld, int vec, int rows, int cols, int cols8, int lcx,
+                                                        const float* __restrict__ z, int act, void* __restrict__ dz, float* __restrict__ part,
+                                                        void* __restrict__ out) {
+    __shared__ float red[256][9];
+    const int cx = threadIdx.x & ((1 << lcx) - 1), ry = threadIdx.x >> lcx, lanes = 256 >> lcx, c = ((blockIdx.x << lcx) + cx) * 8;
     const int per = (rows + gridDim.y - 1) / gridDim.y, r0 = blockIdx.y * per, r1 = r0 + per < rows ? r0 + per : rows;
     float s[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     if (c < cols8)
-        for (int r = r0 + ry; r < r1; r += 8) {
+        for (int r = r0 + ry; r < r1; r += lanes) {
             float v[8];
-            mm_ld8<BF>(x, r * ld + c, v);
+            if constexpr (DZ) {
+                float p[8], a[8], slope[8];
+                mm_row8<BF>(x, r * ld, c, cols, vec != 0, v);
+                mm_ldf8(z + (long long)r * cols8 + c, p);
+                mm_act_slope8(act, p, a, slope);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] *= slope[j];
+                mm_put8<BF>(dz, (long long)r * cols8, c, cols, cols8, true, v);
+            } else mm_ld8<BF>(x, r * ld + c, v);
 #pragma unroll
             for (int j = 0; j < 8; ++j) s[j] += v[j];
         }
+    if (!part && !out) return;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) red[ry][cx][j] = s[j];
+    for (int j = 0; j < 8; ++j) red[threadIdx.x][j] = s[j];
     __syncthreads();
+    const int own = threadIdx.x, col = (blockIdx.x << lcx) * 8 + own;
+    if (own >= (8 << lcx) || col >= cols8) return;
     float t = 0.0f;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) t += red[k][threadIdx.x >> 3][threadIdx.x & 7];
-    const int col = blockIdx.x * 256 + threadIdx.x;
-    if (col < cols8) part[(size_t)blockIdx.y * cols8 + col] = t;
+    for (int k = 0; k < lanes; ++k) t += red[(k << lcx) + (own >> 3)][own & 7];
+    if (part) part[(size_t)blockIdx.y * cols8 + col] = t;
+    else if (col < cols) ((typename MmEl<BF>::T*)out)[col] = (typename MmEl<BF>::T)t;
 }
+// 32 columns a workgroup, 8 lanes a column
 template <bool BF> __global__ __launch_bounds__(256) void mm_colsum_join_kernel(const float* __restrict__ part, int n, int cols8, int cols, void* __restrict__ out) {
-    const int c = blockIdx.x * 256 + threadIdx.x;
-    if (c >= cols) return;
+    __shared__ float red[8][33];
+    const int cx = threadIdx.x & 31, ry = threadIdx.x >> 5, c = blockIdx.x * 32 + cx;
     float t = 0.0f;
-    for (int k = 0; k < n; ++k) t += part[(size_t)k * cols8 + c];
+    if (c < cols)
+        for (int k = ry; k < n; k += 8) t += part[(size_t)k * cols8 + c];
+    red[ry][cx] = t;
+    __syncthreads();
+    if (ry != 0 || c >= cols) return;
+#pragma unroll
+    for (int k = 1; k < 8; ++k) t += red[k][cx];
     ((typename MmEl<BF>::T*)out)[c] = (typename MmEl<BF>::T)t;
 }
 
@@ -119,6 +131,7 @@ struct Arena {
 
 struct Ctx {
     Arena& ar; bool bf; hipStream_t st; int rc = ACMIL_OK;
+    MmPads pads = {};                                                // asked for, not yet launched
     bool go() const { return rc == ACMIL_OK && !ar.dry(); }
     void launched() { if (hipGetLastError() != hipSuccess) rc = ACMIL_ERR_LAUNCH; }
     bool room() { if (ar.full()) { if (rc == ACMIL_OK) rc = ACMIL_ERR_SHAPE; return false; } return true; }
@@ -129,15 +142,24 @@ struct Mat { const void* p; long long ld; int rows, cols; };
 inline bool on16(const void* p) { return ((size_t)p & 15) == 0; }
 inline unsigned grid_of(long long items) { const long long g = (items + 255) / 256; return (unsigned)(g < 1 ? 1 : g > 65536 ? 65536 : g); }
 
+// launch the padding copies asked for so far: in front of the first kernel that reads one
+void flush(Ctx& c) {
+    if (c.pads.count == 0) return;
+    if (c.room() && c.go()) {
+        hipLaunchKernelGGL(mm_pad_kernel, dim3(grid_of(c.pads.total)), dim3(256), 0, c.st, c.pads);
+        c.launched();
+    }
+    c.pads.count = 0;
+    c.pads.total = 0;
+}
 // m as the products take it: rows on 16 bytes, a multiple of 8 columns (zeros behind the last)
 Mat aligned(Ctx& c, const Mat& m, bool force = false) {
     if (!force && on16(m.p) && m.ld % 8 == 0 && m.cols % 8 == 0) return m;
     const int ldd = r8(m.cols);
     short* d = (short*)c.ar.take((size_t)m.rows * ldd * 2);
-    if (c.room() && c.go()) {
-        hipLaunchKernelGGL(mm_pad_kernel, dim3(grid_of((long long)m.rows * (ldd / 8))), dim3(256), 0, c.st, (const short*)m.p, m.ld, m.rows, m.cols, d, ldd);
-        c.launched();
-    }
+    if (c.pads.count == MM_PADS) flush(c);
+    c.pads.m[c.pads.count++] = {(const short*)m.p, d, m.ld, c.pads.total, m.rows, m.cols, ldd};
+    c.pads.total += (long long)m.rows * (ldd / 8);
     return Mat{d, ldd, m.rows, ldd};
 }
 // two matrices that one product addresses with one leading dimension
@@ -163,8 +185,8 @@ void join(Ctx& c, const MmArgs& a, int epi) {
 }
 
 // How many ways to split K of a product of 128 x 128 tiles.  A step of one tile takes about 0.55 us alone on its CU and 1.0 us beside
-// another; a split costs a join launch and 8 bytes of partial sums per output and part, written and read at about 4 TB/s.  Without the
-// second term (split until 512 workgroups) 2000 x 768 x 768 took 20.2 us against 11.1, without a split at all 64 x 4096 x 4096 37 against 14.
+// another; a split costs a join launch and 8 bytes of partial sums per output and part, written and read at about 4 TB/s.  The rule without
+// these costs, as many parts as fill 512 workgroups, took 20.2 us for 2000 x 768 x 768 against 11.2, and 19.4 for 64 x 4096 x 4096 against 15.4.
 int mm_splits(long long tiles, int steps, double outputs) {
     int best = 1;
     double least = 1e30;
@@ -212,6 +234,7 @@ void product(Ctx& c, int kind, MmArgs a, int epi) {
         a.e.ldpart = r8(a.e.npad);
         a.e.part = (float*)c.ar.take((size_t)a.splits * (dual ? 2 : 1) * a.M * a.e.ldpart * 4);
     }
+    flush(c);
     if (c.room() && c.go()) {
         const int e = a.splits > 1 ? MM_PART : epi, cfg = large ? MM_L : slim ? (bm == 32 ? MM_R32 : MM_R64) : tiles * a.splits <= 256 ? MM_D : MM_S;
         c.rc = kind == FWD ? mm_launch_fwd(a, c.bf, e, dual, cfg, c.st) : kind == DGRAD ? mm_launch_dgrad(a, c.bf, e, cfg, c.st)
@@ -234,21 +257,26 @@ void output(MmArgs& a, void* out, long long ldo, const void* bias = nullptr, con
     a.e.vec = on16(out) && ldo % 8 == 0 && on16(bias) && on16(res) && ldr % 8 == 0;      // null is on 16 bytes
 }
 
-void colsum(Ctx& c, const Mat& x, int rows, int cols, void* out) {
+// out [cols] = column sums of x (null: none wanted); with z, x is dy and dz [rows][round8(cols)] receives dy act'(z)
+void colsum(Ctx& c, const Mat& x, int rows, int cols, void* out, const float* z = nullptr, int act = ACMIL_ACT_NONE, void* dz = nullptr) {
     const size_t mark = c.ar.off;
-    const int c8 = r8(cols);
-    int gy = rows / 64;
-    gy = gy < 1 ? 1 : gy > 128 ? 128 : gy;
-    float* part = (float*)c.ar.take((size_t)gy * c8 * 4);
+    const int c8 = r8(cols), vec = on16(x.p) && x.ld % 8 == 0;
+    int lcx = 0;
+    while (lcx < 5 && (8 << lcx) < c8) ++lcx;
+    const int gx = (c8 + (8 << lcx) - 1) / (8 << lcx), lanes = 256 >> lcx, most = gx >= 256 ? 8 : 2048 / gx;
+    int gy = rows / (2 * lanes);                                     // enough workgroups to keep the memory busy, and at least two rows a lane
+    gy = rows <= 8 * lanes ? 1 : gy > most ? most : gy;
+    gy = gy > 256 ? 256 : gy;
+    float* part = out && gy > 1 ? (float*)c.ar.take((size_t)gy * c8 * 4) : nullptr;
+    flush(c);
     if (c.room() && c.go()) {
-        const dim3 g((c8 + 255) / 256, gy), j((cols + 255) / 256);
-        if (c.bf) {
-            hipLaunchKernelGGL((mm_colsum_kernel<true>), g, dim3(256), 0, c.st, x.p, x.ld, rows, c8, part);
-            hipLaunchKernelGGL((mm_colsum_join_kernel<true>), j, dim3(256), 0, c.st, part, gy, c8, cols, out);
-        } else {
-            hipLaunchKernelGGL((mm_colsum_kernel<false>), g, dim3(256), 0, c.st, x.p, x.ld, rows, c8, part);
-            hipLaunchKernelGGL((mm_colsum_join_kernel<false>), j, dim3(256), 0, c.st, part, gy, c8, cols, out);
-        }
+        const dim3 g(gx, gy);
+#define COLSUM(B, Z) hipLaunchKernelGGL((mm_colsum_kernel<B, Z>), g, dim3(256), 0, c.st, x.p, x.ld, vec, rows, cols, c8, lcx, z, act, dz, part, out)
+        if (z) { if (c.bf) COLSUM(true, true); else COLSUM(false, true); }
+        else { if (c.bf) COLSUM(true, false); else COLSUM(false, false); }
+#undef COLSUM
+        if (part && c.bf) hipLaunchKernelGGL((mm_colsum_join_kernel<true>), dim3((cols + 31) / 32), dim3(256), 0, c.st, part, gy, c8, cols, out);
+        else if (part) hipLaunchKernelGGL((mm_colsum_join_kernel<false>), dim3((cols + 31) / 32), dim3(256), 0, c.st, part, gy, c8, cols, out);
         c.launched();
     }
     c.ar.off = mark;
@@ -265,6 +293,7 @@ bool ld_ok(const void* p, long long ld, int cols) { return !p || (ld >= 0 && ld 
 
 void few_rows(Ctx& c, MmArgs a, bool dual) {
     const size_t mark = c.ar.off;
+    flush(c);
     a.splits = mm_rows_splits(a.M, a.e.npad, a.Kq, dual);
     if (a.splits > 1) {
         a.e.ldpart = r8(a.e.npad);
@@ -322,28 +351,23 @@ int linear_bwd(const acmil_linear_args& a, Ctx& c) {
     else {
         const int ldz = r8(a.N);
         void* z = c.ar.take((size_t)a.M * ldz * 2);
-        if (c.room() && c.go()) {
-            const int vec = on16(a.dy) && a.lddy % 8 == 0;
-            const dim3 g(grid_of((long long)a.M * (ldz / 8)));
-            if (c.bf) hipLaunchKernelGGL((mm_dz_kernel<true>), g, dim3(256), 0, c.st, a.dy, a.lddy, vec, a.pre, (long long)ldz, a.act, a.M, a.N, z, ldz);
-            else hipLaunchKernelGGL((mm_dz_kernel<false>), g, dim3(256), 0, c.st, a.dy, a.lddy, vec, a.pre, (long long)ldz, a.act, a.M, a.N, z, ldz);
-            c.launched();
-        }
+        colsum(c, dy, a.M, a.N, a.db, a.pre, a.act, z);
         dz = Mat{z, ldz, a.M, ldz};
     }
+    Mat w{a.W, a.ldw, a.N, a.K}, x{a.x, a.ldx, a.M, a.K};
+    if (a.dx) w = aligned(c, w);
+    if (a.dW) x = aligned(c, x);
     if (a.dx) {
-        const Mat w = aligned(c, Mat{a.W, a.ldw, a.N, a.K});
         MmArgs p = operands(dz, w, a.M, a.K, dz.cols, a.N);
         output(p, a.dx, a.K);
         product(c, DGRAD, p, MM_ACT);
     }
     if (a.dW) {
-        const Mat x = aligned(c, Mat{a.x, a.ldx, a.M, a.K});
         MmArgs p = operands(dz, x, a.N, a.K, a.M, a.M);
         output(p, a.dW, a.K);
         product(c, WGRAD, p, MM_ACT);
     }
-    if (a.db) colsum(c, dz, a.M, a.N, a.db);
+    if (a.db && a.act == ACMIL_ACT_NONE) colsum(c, dz, a.M, a.N, a.db);
     return c.rc;
 }
 
@@ -372,6 +396,8 @@ int ffn_fwd(const acmil_ffn_args& a, Ctx& c) {
     if (!few) { x = aligned(c, x); aligned_pair(c, wg, wu); }
     else if (wg.ld != wu.ld) aligned_pair(c, wg, wu);                // one leading dimension for both
     Mat h{a.h ? a.h : c.ar.take((size_t)a.M * F8 * 2), F8, a.M, F8};
+    const bool few_down = few_rows_wanted(h, wd, 1);
+    if (!few_down) wd = aligned(c, wd);
     if (!c.room()) return c.rc;
     MmArgs p = operands(x, wg, a.M, a.F, few ? a.D : x.cols, few ? a.D : wg.cols);
     p.p1 = (const char*)wu.p;
@@ -380,8 +406,6 @@ int ffn_fwd(const acmil_ffn_args& a, Ctx& c) {
     p.e.bias2 = a.bu; p.e.npad = F8; p.e.act = a.act;
     p.e.pre = a.g; p.e.pre2 = a.u; p.e.ldp = F8;
     if (few) few_rows(c, p, true); else product(c, FWD, p, MM_GATE);
-    const bool few_down = few_rows_wanted(h, wd, 1);
-    if (!few_down) wd = aligned(c, wd);
     MmArgs d = operands(h, wd, a.M, a.D, few_down ? a.F : F8, few_down ? a.F : wd.cols);
     output(d, a.y, a.ldy, a.bd, a.res, a.ldr);
     if (few_down) few_rows(c, d, false); else product(c, FWD, d, MM_ACT);
@@ -391,10 +415,12 @@ int ffn_fwd(const acmil_ffn_args& a, Ctx& c) {
 int ffn_bwd(const acmil_ffn_args& a, Ctx& c) {
     const int F8 = r8(a.F);
     const Mat dy = aligned(c, Mat{a.dy, a.lddy, a.M, a.D}), h{a.h, F8, a.M, F8};
-    Mat x{a.x, a.ldx, a.M, a.D};
+    Mat x{a.x, a.ldx, a.M, a.D}, wg{a.Wg, a.ldwg, a.F, a.D}, wu{a.Wu, a.ldwu, a.F, a.D}, wd{a.Wd, a.ldwd, a.D, a.F};
     Mat dgu{nullptr, 2LL * F8, a.M, 2 * F8};                         // [dg | du], each with zeros behind column F
+    if (a.dx || a.dWgu || a.dbgu) wd = aligned(c, wd);
+    if (a.dx) aligned_pair(c, wg, wu);
+    if (a.dWgu) x = aligned(c, x);
     if (a.dx || a.dWgu || a.dbgu) {
-        const Mat wd = aligned(c, Mat{a.Wd, a.ldwd, a.D, a.F});
         dgu.p = c.ar.take((size_t)a.M * 2 * F8 * 2);
         if (!c.room()) return c.rc;
         MmArgs p = operands(dy, wd, a.M, a.F, dy.cols, a.D);
@@ -404,8 +430,6 @@ int ffn_bwd(const acmil_ffn_args& a, Ctx& c) {
         product(c, DGRAD, p, MM_GATE_BWD);
     }
     if (a.dx) {
-        Mat wg{a.Wg, a.ldwg, a.F, a.D}, wu{a.Wu, a.ldwu, a.F, a.D};
-        aligned_pair(c, wg, wu);
         MmArgs p = operands(dgu, wg, a.M, a.D, F8, a.F);             // dg Wg + du Wu: two K segments of one product
         p.segs = 2;
         p.q1 = p.q0 + 2LL * F8; p.p1 = (const char*)wu.p;
@@ -413,7 +437,6 @@ int ffn_bwd(const acmil_ffn_args& a, Ctx& c) {
         product(c, DGRAD, p, MM_ACT);
     }
     if (a.dWgu) {
-        x = aligned(c, x);
         MmArgs p = operands(dgu, x, 2 * F8, a.D, a.M, a.M);
         output(p, a.dWgu, a.D);
         product(c, WGRAD, p, MM_ACT);

@@ -603,7 +603,7 @@ int acmil_adamw_step_peer(float* params, float* exp_avg, float* exp_avg_sq, long
  *   acmil_linear_act      y [M,N] = act(x W^T + bias) + res        x [M,K], W [N,K], bias [N] or NULL, res [M,N] or NULL (ldr)
  *     pre: NULL, or fp32 [M][round8(N)] (16-byte aligned) that receives x W^T + bias for the backward (act != NONE needs it)
  *   acmil_linear_act_bwd  dz = dy act'(pre); dx [M,K] = dz W, dW [N,K] = dz^T x, db [N] = column sums of dz (each may be NULL; dense);
- *     dz is held in the tensors' type.  The gradient of res is dy itself.
+ *     dz is held in the tensors' type for the products (db sums it before that rounding).  The gradient of res is dy itself.
  *   acmil_gated_ffn       h = act(x Wg^T + bg) * (x Wu^T + bu);  y [M,D] = h Wd^T + bd + res    x [M,D], Wg, Wu [F,D], Wd [D,F]
  *     h is held in the tensors' type.  g, u (fp32 [M][round8(F)]) and h ([M][round8(F)] of dtype), 16-byte aligned: kept for the
  *     backward, all three or none (h then lives in the workspace).

@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from acmil_amd import ops
+from acmil_amd import autograd, ops
 from acmil_amd.optim import FlatAdamW, FlatMuon
 from test_ortho_gpu import iterate
 
@@ -119,6 +119,44 @@ def test_more_matrices_than_one_launch_holds():
         o = ops.orthogonalize(params[k].grad)
         want = start[k] - 1e-2 * 0.2 * math.sqrt(max(params[k].shape)) * o
         assert (params[k] - want).abs().max() <= 2 ** -22 * (start[k].abs().max() + 0.1)       # two roundings of values below 0.6
+
+
+def test_trains_the_16_bit_layers():
+    """a residual block of linear_act and gated_ffn on bf16 copies of fp32 parameters, stepped by FlatMuon: the step is the formula's for the gradients
+    that arrived (bounds as in test_steps_follow_the_formula), and those are the ones the block gives without the optimizer"""
+    g = torch.Generator().manual_seed(3)
+    shapes = {"w": (64, 96), "b": (64,), "wg": (160, 64), "wu": (160, 64), "wd": (64, 160)}
+    p = {k: torch.nn.Parameter((torch.randn(*s, generator=g) * 0.1).cuda()) for k, s in shapes.items()}
+    x, dy = torch.randn(300, 96, generator=g).cuda().bfloat16(), torch.randn(300, 64, generator=g).cuda().bfloat16()
+
+    def block(q):
+        h = autograd.linear_act(x, q["w"], bias=q["b"], act="gelu")
+        return autograd.gated_ffn(h, q["wg"], q["wu"], q["wd"], residual=h)
+
+    opt = FlatMuon(p.values(), lr=1e-2, weight_decay=0.1)
+    for step in range(2):
+        half = {k: v.detach().bfloat16().requires_grad_() for k, v in p.items()}
+        want = torch.autograd.grad(block(half), list(half.values()), dy)
+        before = {k: v.detach().double() for k, v in p.items()}
+        buf = {k: opt.exp_avg[o:o + v.numel()].view(v.shape).double() for (k, v), o in zip(p.items(), _offsets(p))}
+        opt.zero_grad()
+        block({k: v.bfloat16() for k, v in p.items()}).backward(dy)
+        for (k, v), w in zip(p.items(), want):
+            assert torch.equal(v.grad, w.float()), k
+        opt.step()
+        for k in ("w", "wg", "wu", "wd"):
+            grad = p[k].grad.double()
+            o, bound = iterate(grad + 0.95 * (0.95 * buf[k] + grad), torch.float64)
+            scale = 1e-2 * 0.2 * math.sqrt(max(shapes[k]))
+            new = before[k] * (1 - 1e-3) - scale * o
+            assert (p[k].double() - new).norm() <= scale * (bound + 3.9 ** 5 * 2 ** -22) + 8 * 2 ** -24 * float(new.norm()), (step, k)
+
+
+def _offsets(p):
+    at = 0
+    for v in p.values():
+        yield at
+        at += v.numel()
 
 
 @pytest.mark.parametrize("n_token, bags", [(5, 1), (1, 1), (5, 4)])
