@@ -12,7 +12,8 @@
 // second lo.  K is padded to a multiple of 32 with zeros, so there is no tail.  All three products take both operands with K
 // contiguous: X is kept in both orientations (its transpose twice, read and written alternately).  A and B are symmetric: only tiles on
 // and below the diagonal are computed and each is written a second time, mirrored.
-// All matrices of a call go through the same launches: 2 + 3 steps of them, whatever the number of matrices (up to NS_GROUP at a time).
+// All matrices of a call go through the same launches: 2 + 3 steps of them, whatever the number of matrices (up to NS_GROUP at a time); where
+// all are small, one launch does everything (ns_tiny_kernel).
 #include "mm16_kernel.h"
 
 #include <cmath>
@@ -67,8 +68,8 @@ template <int DT> __device__ __forceinline__ void ns_load8(const void* p, long l
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = c + j < cols ? ns_load<DT>(p, row + c + j) : 0.0f;
 }
-template <int DT> __device__ __forceinline__ bool ns_on16(const NsMat& m) {
-    return ((size_t)m.g & 15) == 0 && m.ldg % (DT == ACMIL_DTYPE_F32 ? 4 : 8) == 0;
+template <int DT> __device__ __forceinline__ bool ns_on16(const void* g, long long ldg) {
+    return ((size_t)g & 15) == 0 && ldg % (DT == ACMIL_DTYPE_F32 ? 4 : 8) == 0;
 }
 
 // sum of squares, in 64 bits (a gradient's squares leave the range of 32): NS_PARTS partial sums per matrix, fixed order
@@ -76,7 +77,7 @@ template <int DT> __device__ __forceinline__ bool ns_on16(const NsMat& m) {
 template <int DT> __global__ __launch_bounds__(256) void ns_norm_kernel(NsArgs a, double* part) {
     const NsMat& m = a.m[blockIdx.y];
     const int rows = m.tall ? m.t : m.s, cols = m.tall ? m.s : m.t, cpr = (cols + 7) / 8;
-    const bool vec = ns_on16<DT>(m);
+    const bool vec = ns_on16<DT>(m.g, m.ldg);
     const long long total = (long long)rows * cpr, step = NS_PARTS * 256LL;
     double s = 0.0;
     for (long long i = blockIdx.x * 256LL + threadIdx.x; i < total; i += 2 * step) {
@@ -124,7 +125,7 @@ template <int DT> __global__ __launch_bounds__(256) void ns_split_kernel(NsArgs 
     const int rows = m.tall ? m.t : m.s, cols = m.tall ? m.s : m.t;
     const int ct = (cols + 63) / 64, id = blockIdx.x - a.first[mi], r0 = id / ct * 64, c0 = id % ct * 64;
     float in[2][8];
-    const bool vec = ns_on16<DT>(m);
+    const bool vec = ns_on16<DT>(m.g, m.ldg);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const int r = r0 + (threadIdx.x >> 3) + 32 * h, c = c0 + (threadIdx.x & 7) * 8;
@@ -373,6 +374,246 @@ __global__ __launch_bounds__(C::WAVES * KG * 64) void ns_kernel(NsArgs a) {
         }
 }
 
+// Small matrices, whole iterations in one workgroup.  Where X, both halves, and one s x s matrix fit the 160 KB of LDS (64 x 512, 128 x 160),
+// a call of 2 + 3 steps dependent launches is nothing but their latencies.  Here a workgroup loads its matrix once (through registers: the norm is
+// formed on the way), keeps X in LDS and multiplies there: A = X X^T from rows of X, B over A, X <- a X + B X in place (32 columns are a wave's
+// own: it holds them as fragments before it writes).  X is its own transpose, read by ds_read_b64_tr_b16.  Rows are padded by 16 bytes: their
+// length in banks is then an odd multiple of 4, and 16 rows of 16 bytes meet no bank twice.  Same arithmetic, same roundings as the tiles.
+//
+// (a on the diagonal of B would save reading X back, but rounds a X once more: 5 times the error of an fp32 iteration for a rank-one matrix.)
+// A step of 64 x 512 takes about 10 us, half of it matrix instructions and LDS reads, half the epilogues' conversions.  Against the tiles:
+// 16 x 16 11 us (65), 64 x 64 23 (73), 64 x 512 54 (87), 128 x 160 64 (90), sixty of 128 x 128 56 (325).
+#define NS_TINY 60                // matrices of a launch: what the kernel arguments hold
+#define NS_TINY_LDS (160 * 1024 - 64)
+#define NS_TINY_CHUNKS 10         // of 8 values per thread: s t <= 40 000
+#define NS_MAX_STEPS 64
+
+struct NsTinyMat { const void* g; void* o; long long ldg, ldo; int s, t, tall, pad; };
+struct NsTiny {
+    int steps; float eps;
+    float co[3 * NS_MAX_STEPS];
+    NsTinyMat m[NS_TINY];
+};
+// bytes behind X: A, or the partial tiles of one round of a sum
+__host__ __device__ constexpr long long ns_tiny_square(int S) { return S == 32 ? 12 * 1024 : S * (S + 8) * 4LL; }
+__host__ __device__ static inline bool ns_tiny_fits(int s, int t) {
+    const long long S = ns_r32(s), T = ns_r32(t);
+    return S <= 128 && S * (T + 8) * 4 + ns_tiny_square((int)S) <= NS_TINY_LDS;
+}
+__device__ __forceinline__ void ns_tiny_put(short* h, short* l, f32x4 v) {
+    unsigned hi[2], lo[2];
+    ga_split_pair_f16(v[0], v[1], hi[0], lo[0]);
+    ga_split_pair_f16(v[2], v[3], hi[1], lo[1]);
+    *(uint2*)h = uint2{hi[0], hi[1]};
+    *(uint2*)l = uint2{lo[0], lo[1]};
+}
+// acc += c (hi + lo)
+__device__ __forceinline__ void ns_tiny_add(f32x4& acc, float c, const short* h, const short* l) {
+    typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+    const h4 x = *(const h4*)h, y = *(const h4*)l;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] = fmaf((float)x[e], c, fmaf((float)y[e], c, acc[e]));
+}
+
+// the iterations; SK = padded s / 32
+template <int DT, int SK> struct NsTinyRun {
+    static constexpr int S = 32 * SK, LDA = S + 8, UNITS = SK * SK, PER_WAVE = (UNITS + 7) / 8;           // units of 32 x 32 of an s x s matrix
+    static constexpr int KSPLIT = SK == 1 ? 4 : SK == 2 ? 2 : 1;      // ways K of X X^T is split over waves
+    static_assert((KSPLIT - 1) * UNITS * 4096 <= ns_tiny_square(S), "partial sums lie over A");
+
+    // A = X X^T, or (POLY; h, l are A) B = cb A + cc A A over A.  A is symmetric: its rows are its columns
+    template <int KS, bool POLY> static __device__ __forceinline__ void square(const short* h, const short* l, int ld, int K, short* Ah, float cb, float cc) {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, kg = lane >> 4, kq = KS == 1 ? 0 : wave / UNITS;
+        short* Al = Ah + S * LDA;
+        f32x4 acc[PER_WAVE][2][2] = {};
+#pragma unroll
+        for (int w = 0; w < PER_WAVE; ++w) {
+            const int u = KS == 1 ? wave + 8 * w : wave % UNITS, m0 = u / SK * 32, n0 = u % SK * 32;
+            if (u >= UNITS || kq >= KS) continue;
+            const int q = (m0 + r) * ld + 8 * kg, p = (n0 + r) * ld + 8 * kg;
+            for (int k = 32 * kq; k < K; k += 32 * KS) {
+                s16x8 ph[2], pl[2], qh[2], ql[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    ph[i] = *(const s16x8*)(h + p + 16 * i * ld + k); pl[i] = *(const s16x8*)(l + p + 16 * i * ld + k);
+                    qh[i] = *(const s16x8*)(h + q + 16 * i * ld + k); ql[i] = *(const s16x8*)(l + q + 16 * i * ld + k);
+                }
+#pragma unroll
+                for (int o = 0; o < 3; ++o)                           // the small products first
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) acc[w][i][j] = mm_mfma<false>(o == 0 ? pl[j] : ph[j], o == 1 ? ql[i] : qh[i], acc[w][i][j]);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const int m = m0 + 16 * i + r, n = n0 + 16 * j + 4 * kg;
+                    acc[w][i][j] *= POLY ? cc / NS_SCALE : 1.0f / NS_SCALE;
+                    if (POLY) ns_tiny_add(acc[w][i][j], cb, Ah + m * LDA + n, Al + m * LDA + n);
+                }
+        }
+        if (POLY) __syncthreads();                                    // everybody has read A
+        if (KS > 1 && K > 32) {
+            f32x4* part = (f32x4*)Ah + (wave % UNITS) * 256 + lane;   // [kq - 1][unit][tile][lane]
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (kq > 0 && kq < KS) part[((kq - 1) * UNITS * 4 + i) * 64] = acc[0][i >> 1][i & 1];
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k + 1 < KS; ++k)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (kq == 0) acc[0][i >> 1][i & 1] += part[(k * UNITS * 4 + i) * 64];
+            __syncthreads();
+        }
+#pragma unroll
+        for (int w = 0; w < PER_WAVE; ++w) {
+            const int u = KS == 1 ? wave + 8 * w : wave % UNITS, at = (u / SK * 32 + r) * LDA + u % SK * 32 + 4 * kg;
+            if (u >= UNITS || kq > 0) continue;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) ns_tiny_put(Ah + at + 16 * i * LDA + 16 * j, Al + at + 16 * i * LDA + 16 * j, acc[w][i][j]);
+        }
+        __syncthreads();
+    }
+
+    static __device__ __forceinline__ void run(const NsTiny& a, const NsTinyMat& m, char* smem) {
+        const int T = ns_r32(m.t), ldx = T + 8, wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r = lane & 15, kg = lane >> 4;
+        short *Xh = (short*)smem, *Xl = Xh + S * ldx, *Ah = Xl + S * ldx, *Al = Ah + S * LDA;
+        mm_lds* const lds = (mm_lds*)smem;
+        const unsigned xl = S * ldx * 2;
+        const unsigned turn = ((8 * kg + (r >> 2)) * ldx + 4 * (lane & 3)) * 2;                  // of a K-strided fragment: MmFrag, without a permutation
+        auto frag = [&](mm_lds* q) MM_INLINE {
+            const s16x4 x = __builtin_bit_cast(s16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) mm_h4*)q));
+            const s16x4 y = __builtin_bit_cast(s16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) mm_h4*)(q + 8 * ldx)));
+            return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+        };
+        for (int step = 0; step < a.steps; ++step) {
+            const float ca = a.co[3 * step];
+            square<KSPLIT, false>(Xh, Xl, ldx, T, Ah, 0.0f, 0.0f);
+            square<1, true>(Ah, Al, LDA, S, Ah, a.co[3 * step + 1], a.co[3 * step + 2]);
+            // X <- a X + B X.  B, up to 64 x 64, is read once for all columns of a wave
+            constexpr bool HELD = SK <= 2;
+            s16x8 qh[HELD ? 2 * SK : 1][SK], ql[HELD ? 2 * SK : 1][SK];
+            if constexpr (HELD)
+#pragma unroll
+                for (int i = 0; i < 2 * SK; ++i)
+#pragma unroll
+                    for (int k = 0; k < SK; ++k) {
+                        qh[i][k] = *(const s16x8*)(Ah + (16 * i + r) * LDA + 32 * k + 8 * kg);
+                        ql[i][k] = *(const s16x8*)(Al + (16 * i + r) * LDA + 32 * k + 8 * kg);
+                    }
+            // (the last step, with its bounds on what is stored, is a copy of its own: branches between the tiles keep them from overlapping)
+            auto columns = [&](int n0, auto last) MM_INLINE {
+                s16x8 ph[SK][2], pl[SK][2];
+#pragma unroll
+                for (int k = 0; k < SK; ++k)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        mm_lds* p = lds + turn + (32 * k * ldx + n0 + 16 * j) * 2;
+                        ph[k][j] = frag(p);
+                        pl[k][j] = frag(p + xl);
+                    }
+                auto rows = [&](int i, const s16x8* bh, const s16x8* bl) MM_INLINE {
+                    f32x4 acc[2] = {};
+#pragma unroll
+                    for (int k = 0; k < SK; ++k)
+#pragma unroll
+                        for (int p = 0; p < 3; ++p)
+#pragma unroll
+                            for (int j = 0; j < 2; ++j) acc[j] = mm_mfma<false>(p == 0 ? pl[k][j] : ph[k][j], p == 1 ? bl[k] : bh[k], acc[j]);
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const int mr = 16 * i + r, n = n0 + 16 * j + 4 * kg, at = mr * ldx + n;
+                        f32x4 v = acc[j] * (1.0f / NS_SCALE);
+                        ns_tiny_add(v, ca, Xh + at, Xl + at);
+                        if constexpr (!decltype(last)::value) ns_tiny_put(Xh + at, Xl + at, v);
+                        else if (mr < m.s)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                if (n + e < m.t) ns_store<DT>(m.o, m.tall ? (n + e) * m.ldo + mr : mr * m.ldo + n + e, v[e] * (1.0f / NS_SCALE));
+                    }
+                };
+                if constexpr (HELD) {
+#pragma unroll
+                    for (int i = 0; i < 2 * SK; ++i) rows(i, qh[i], ql[i]);
+                } else {
+                    for (int i = 0; i < 2 * SK; ++i) {
+#pragma unroll
+                        for (int k = 0; k < SK; ++k) {
+                            qh[0][k] = *(const s16x8*)(Ah + (16 * i + r) * LDA + 32 * k + 8 * kg);
+                            ql[0][k] = *(const s16x8*)(Al + (16 * i + r) * LDA + 32 * k + 8 * kg);
+                        }
+                        rows(i, qh[0], ql[0]);
+                    }
+                }
+            };
+            if (step + 1 < a.steps)
+                for (int n0 = wave * 32; n0 < T; n0 += 256) columns(n0, std::false_type());
+            else
+                for (int n0 = wave * 32; n0 < T; n0 += 256) columns(n0, std::true_type());
+            __syncthreads();
+        }
+    }
+};
+
+template <int DT> __global__ __launch_bounds__(512, 2) void ns_tiny_kernel(NsTiny a) {
+    __shared__ __attribute__((aligned(128))) char smem[NS_TINY_LDS];
+    __shared__ double red[8];
+    const NsTinyMat& m = a.m[blockIdx.x];
+    const int S = ns_r32(m.s), T = ns_r32(m.t), ldx = T + 8, total = S * T / 8;
+    const int rows = m.tall ? m.t : m.s, cols = m.tall ? m.s : m.t, cpr = (m.tall ? S : T) / 8;
+    const bool vec = ns_on16<DT>(m.g, m.ldg);
+    float v[NS_TINY_CHUNKS][8];
+    double sum = 0.0;
+#pragma unroll
+    for (int h = 0; h < NS_TINY_CHUNKS; ++h) {
+        const int i = threadIdx.x + 512 * h, q = i / cpr, c = (i - q * cpr) * 8;
+        if (i < total && q < rows && c < cols) ns_load8<DT>(m.g, q * m.ldg, c, cols, vec, v[h]);
+        else
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[h][j] = 0.0f;
+    }
+#pragma unroll
+    for (int h = 0; h < NS_TINY_CHUNKS; ++h)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum += (double)v[h][j] * (double)v[h][j];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = sum;
+    __syncthreads();
+    sum = ((red[0] + red[1]) + (red[2] + red[3])) + ((red[4] + red[5]) + (red[6] + red[7]));
+    const double scale = (double)NS_SCALE / (sqrt(sum) + (double)a.eps);
+    short *Xh = (short*)smem, *Xl = Xh + S * ldx;
+#pragma unroll
+    for (int h = 0; h < NS_TINY_CHUNKS; ++h) {
+        const int i = threadIdx.x + 512 * h, q = i / cpr, c = (i - q * cpr) * 8;
+        if (i < total) {
+            unsigned hi[4], lo[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) ga_split_pair_f16((float)((double)v[h][2 * j] * scale), (float)((double)v[h][2 * j + 1] * scale), hi[j], lo[j]);
+            if (!m.tall) {
+                *(u32x4*)(Xh + q * ldx + c) = u32x4{hi[0], hi[1], hi[2], hi[3]};
+                *(u32x4*)(Xl + q * ldx + c) = u32x4{lo[0], lo[1], lo[2], lo[3]};
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    Xh[(c + j) * ldx + q] = (short)(hi[j >> 1] >> (16 * (j & 1)));
+                    Xl[(c + j) * ldx + q] = (short)(lo[j >> 1] >> (16 * (j & 1)));
+                }
+            }
+        }
+    }
+    __syncthreads();
+    if (S == 32) NsTinyRun<DT, 1>::run(a, m, smem);
+    else if (S == 64) NsTinyRun<DT, 2>::run(a, m, smem);
+    else if (S == 96) NsTinyRun<DT, 3>::run(a, m, smem);
+    else NsTinyRun<DT, 4>::run(a, m, smem);
+}
+
 namespace {
 
 typedef MmGeom<64, 64, 4, 2> NsT;
@@ -418,7 +659,32 @@ template <int KIND, int DT> int ns_product(NsArgs& a, hipStream_t st) {
     return ns_go<NsT, 2, 1, KIND, DT>(a, st);
 }
 
+// all matrices small: one launch for NS_TINY of them (beside a larger one they would add a launch to those that they can share)
+bool ns_tiny_call(int count, const acmil_ortho_mat* mats) {
+    for (int i = 0; i < count; ++i)
+        if (!ns_tiny_fits(mats[i].m < mats[i].n ? mats[i].m : mats[i].n, mats[i].m < mats[i].n ? mats[i].n : mats[i].m)) return false;
+    return true;
+}
+template <int DT> int ns_tiny_go(int count, const acmil_ortho_mat* mats, int steps, const float* co, float eps, hipStream_t st) {
+    for (int at = 0; at < count; at += NS_TINY) {
+        NsTiny a = {};
+        const int n = count - at < NS_TINY ? count - at : NS_TINY;
+        a.steps = steps;
+        a.eps = eps;
+        for (int k = 0; k < 3 * steps; ++k) a.co[k] = co[k];
+        for (int i = 0; i < n; ++i) {
+            const acmil_ortho_mat& u = mats[at + i];
+            const int tall = u.m > u.n;
+            a.m[i] = {u.g, u.o, u.ldg, u.ldo, tall ? u.n : u.m, tall ? u.m : u.n, tall, 0};
+        }
+        hipLaunchKernelGGL((ns_tiny_kernel<DT>), dim3(n), dim3(512), 0, st, a);
+        if (hipGetLastError() != hipSuccess) return ACMIL_ERR_LAUNCH;
+    }
+    return ACMIL_OK;
+}
+
 template <int DT> int ns_run(int count, const acmil_ortho_mat* mats, int steps, const float* co, float eps, char* ws, hipStream_t st) {
+    if (ns_tiny_call(count, mats)) return ns_tiny_go<DT>(count, mats, steps, co, eps, st);
     for (int at = 0; at < count; at += NS_GROUP) {                   // groups reuse the workspace: stream order
         NsArgs a = {};
         a.count = count - at < NS_GROUP ? count - at : NS_GROUP;
@@ -454,7 +720,7 @@ template <int DT> int ns_run(int count, const acmil_ortho_mat* mats, int steps, 
     return ACMIL_OK;
 }
 
-const int NS_MAX_DIM = 1 << 16, NS_MAX_STEPS = 64;
+const int NS_MAX_DIM = 1 << 16;
 
 int ns_check(int count, const acmil_ortho_mat* mats, int dtype) {
     if (!mats) return ACMIL_ERR_NULL;

@@ -50,6 +50,29 @@ def test_sizes(m, n, dt):
     check(ops.orthogonalize(gradient(m, n, DTS[dt], seed=m)), gradient(m, n, DTS[dt], seed=m))
 
 
+@pytest.mark.parametrize("m, n", [(16, 40), (32, 1152), (32, 1185), (1150, 19), (50, 544), (64, 545), (96, 288), (70, 289), (271, 90), (128, 160), (101, 160), (128, 161), (150, 128)])
+@pytest.mark.parametrize("dt", list(DTS))
+def test_matrices_that_fit_one_workgroup_and_just_do_not(m, n, dt):
+    g = gradient(m, n, DTS[dt], seed=n)
+    check(ops.orthogonalize(g), g)
+    many = torch.stack([gradient(m, n, DTS[dt], seed=n + k) for k in range(3)])
+    got = ops.orthogonalize(many)
+    assert torch.equal(got[0], ops.orthogonalize(g)) and torch.equal(got, ops.orthogonalize(many)) and torch.equal(ops.orthogonalize(many, out=many), got)
+
+
+def test_small_matrices_of_all_shapes_in_one_call():
+    shapes = [(1, 7), (200, 30), (64, 64), (128, 160), (96, 3), (33, 400), (90, 90)] * 19                   # more than two launches hold
+    gs = [gradient(*s, torch.float32, seed=k % 7) for k, s in enumerate(shapes)]
+    wide = torch.full((64, 100), 7.0, device="cuda")
+    wide[:, 3:67] = gs[2]
+    gs[2] = wide[:, 3:67]                                                                                  # rows on 4 bytes
+    outs = ops.orthogonalize(gs)
+    for k in list(range(7)) + [58, 59, 60, 61, 119, 120, 132]:
+        check(outs[k], gs[k])
+        assert torch.equal(outs[k], outs[k % 7])
+    check(ops.orthogonalize(gs[3], steps=9, coeffs=(1.5, -0.5, 0.0)), gs[3], steps=9, coeffs=(1.5, -0.5, 0.0))
+
+
 @pytest.mark.parametrize("m, n", [(1500, 1900), (2900, 2700)])
 def test_larger_tiles(m, n):
     g = gradient(m, n, torch.float32)
