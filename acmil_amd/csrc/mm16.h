@@ -48,14 +48,33 @@ template <bool BF> struct MmEl;
 template <> struct MmEl<true> { typedef __bf16 T; typedef bf16x8 V; };
 template <> struct MmEl<false> { typedef _Float16 T; typedef f16x8 V; };
 
-// sigmoid with one exponential; exp overflows to inf for very negative z and the quotient is then exactly 0
-__device__ __forceinline__ float mm_sigmoid(float z) { return 1.0f / (1.0f + __expf(-z)); }
+// An epilogue evaluates these for every output, and on the vector unit of a CU that is no small part of a call: with the library's erff and an
+// IEEE division a GELU layer of 768 rows took 3 us more than one without an activation, whatever its K.
+// Sigmoid: one exponential, one reciprocal (1 ulp); exp overflows to inf for very negative z and the result is then exactly 0.
+__device__ __forceinline__ float mm_sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + __expf(-z)); }
+
+// Normal distribution function, e = exp(-z^2 / 2).  Phi(-x) = e P(t), t = 1 / (1 + 0.3 x): the form of Abramowitz and Stegun 7.1.26 with a
+// degree-8 P fitted to least relative error over 0 <= x <= 14 (1.5e-7; in fp32: 6e-7 for x < 3, absolute 7e-8, and no loss in the lower tail).
+__device__ __forceinline__ float mm_normal_cdf(float z, float& e) {
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.3f, fabsf(z), 1.0f));
+    float p = 0.03567476198f;
+    p = fmaf(p, t, -0.15720301867f);
+    p = fmaf(p, t, 0.20635335147f);
+    p = fmaf(p, t, -0.05368350446f);
+    p = fmaf(p, t, 0.12856155634f);
+    p = fmaf(p, t, 0.09991351516f);
+    p = fmaf(p, t, 0.12075395882f);
+    p = fmaf(p, t, 0.11962930113f);
+    e = __expf(-0.5f * z * z);
+    const float q = p * t * e;
+    return z < 0.0f ? q : 1.0f - q;                                       // NaN stays NaN
+}
 
 __device__ __forceinline__ float mm_act(int act, float z) {
     switch (act) {
         case ACMIL_ACT_RELU: return z < 0.0f ? 0.0f : z;                 // NaN stays NaN
         case ACMIL_ACT_SILU: return z * mm_sigmoid(z);
-        case ACMIL_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+        case ACMIL_ACT_GELU: { float e; return z * mm_normal_cdf(z, e); }
         case ACMIL_ACT_GELU_TANH: return z * mm_sigmoid(1.5957691216057308f * (z + 0.044715f * z * z * z));   // 0.5 z (1 + tanh t) = z sigmoid(2 t)
         case ACMIL_ACT_SIGMOID: return mm_sigmoid(z);
         default: return z;
@@ -68,8 +87,9 @@ __device__ __forceinline__ float mm_act_slope(int act, float z, float& slope) {
         case ACMIL_ACT_RELU: slope = z > 0.0f ? 1.0f : 0.0f; return z < 0.0f ? 0.0f : z;
         case ACMIL_ACT_SILU: { const float s = mm_sigmoid(z); slope = s * (1.0f + z * (1.0f - s)); return z * s; }
         case ACMIL_ACT_GELU: {
-            const float c = 0.5f * (1.0f + erff(z * 0.70710678118654752f));
-            slope = c + z * 0.39894228040143268f * __expf(-0.5f * z * z);
+            float e;
+            const float c = mm_normal_cdf(z, e);
+            slope = c + z * 0.39894228040143268f * e;
             return z * c;
         }
         case ACMIL_ACT_GELU_TANH: {
