@@ -5,13 +5,16 @@
 // dW = dz^T x: P = x (KS), Q = dz (KS).  DUAL multiplies the same Q by two P (gate and up projection) so that one wave holds both
 // factors of an output element in its accumulators and the product needs no second pass.
 //
-// Layout.  A K step is 64 wide.  Tiles travel global -> LDS by 16-byte LDS-DMA (no registers) through a ring, one barrier a
-// step.  The LDS image is linear in the DMA's lane order, so bank
-// conflicts are avoided by permuting which 16-byte chunk of its row each LANE FETCHES.  K-strided tiles lie in LDS as they lie in
-// memory ([k][row]) and are read by ds_read_b64_tr_b16, which hands every lane four consecutive k of its row: no transposed copy of
+// Layout.  A K step is 64 wide.  Tiles travel global -> LDS by 16-byte LDS-DMA (no registers) through a ring, one barrier a step.  The
+// LDS image is linear in the DMA's lane order, so bank conflicts are avoided by permuting which 16-byte chunk of its row each LANE
+// FETCHES.  K-strided tiles lie in LDS as they lie in memory ([k][row]) and are read by ds_read_b64_tr_b16, which hands every lane four consecutive k of its row: no transposed copy of
 // an operand is ever made.  P feeds the A side of the instruction: a lane then owns 4 consecutive COLUMNS of an output row.
 // The epilogue turns the accumulators through LDS (fp32, 68-float rows: conflict-free both ways) into 8 consecutive columns per
 // lane, so bias, residual, saved values and the result move in 16-byte pieces, 128 bytes a row.
+//
+// Bound: large products by the card's power (8192 x 4096 x 11008 training block 5.3 ms, 1.25 PFLOP/s over its nine products and its
+// element-wise work; a library product of 4096^3 1.45), small ones by latency: a call of 768 x 2816 outputs takes 6 us for K = 64 and 0.45 us for
+// every further step, an activation 1 to 2 us.
 #pragma once
 #include "mm16.h"
 
@@ -165,7 +168,7 @@ __global__ __launch_bounds__(MmCfg<CFG>::WAVES * 64, MmCfg<CFG>::PER_SIMD) void 
     const unsigned smem0 = mm_lds_addr(smem);
 
     // Fetching one operand of one step in NI pieces.  Fetches are never skipped, so that their count is a constant: behind the last step
-    // it is fetched again, unused.  TAIL (a K that is no multiple of 64): chunks beyond K come from the zero block.
+    // it is fetched again, unused.  tail (a K that is no multiple of 64): chunks beyond K come from the zero block.
     constexpr int NIQ = decltype(lq)::NI, NIP = decltype(lp)::NI;
     struct Half { const char *from, *from2; unsigned lds; int k; };  // k: how much of K is left
     auto half_of = [&](int t, int slot, bool rows) MM_INLINE {
@@ -221,7 +224,15 @@ __global__ __launch_bounds__(MmCfg<CFG>::WAVES * 64, MmCfg<CFG>::PER_SIMD) void 
         q[f] = fq.get(slot, 16 * f, sub);
     };
     mm_lds* const ring = (mm_lds*)smem;
-    auto run = [&](auto tail) MM_INLINE {
+    int qs = 0, ps = 0;                                              // slots of Q_t and P_t
+    auto start = [&](auto tail) MM_INLINE {
+        mm_for<0, D>([&](auto i) MM_INLINE {
+            const Half hq = half_of(t0 + i, i, true), hp = half_of(t0 + i, i, false);
+            mm_for<0, NIQ>([&](auto d) MM_INLINE { fetch_q(hq, d, tail); });
+            mm_for<0, NIP>([&](auto d) MM_INLINE { fetch_p(hp, d, tail); });
+        });
+    };
+    auto steps = [&](int from, int to, auto tail) MM_INLINE {
         // piece `sub` multiplies; fragments of the other piece are read from the given slots
         auto piece = [&](auto ks, mm_lds* qslot, mm_lds* pslot, const Half& h) MM_INLINE {
             constexpr int sub = decltype(ks)::value;
@@ -238,17 +249,7 @@ __global__ __launch_bounds__(MmCfg<CFG>::WAVES * 64, MmCfg<CFG>::PER_SIMD) void 
                 __builtin_amdgcn_sched_barrier(0);
             });
         };
-        mm_for<0, D>([&](auto i) MM_INLINE {
-            const Half hq = half_of(t0 + i, i, true), hp = half_of(t0 + i, i, false);
-            mm_for<0, NIQ>([&](auto d) MM_INLINE { fetch_q(hq, d, tail); });
-            mm_for<0, NIP>([&](auto d) MM_INLINE { fetch_p(hp, d, tail); });
-        });
-        mm_wait_dma<(D - 1) * (NIQ + NIP)>();
-        ga_lds_barrier();
-        int qs = 0, ps = 0;                                          // slots of Q_t and P_t
-        mm_for<0, NT>([&](auto f) MM_INLINE { read_p(ring + RINGP, std::integral_constant<int, 0>{}, f); });
-        mm_for<0, MT>([&](auto f) MM_INLINE { read_q(ring, std::integral_constant<int, 0>{}, f); });
-        for (int t = t0; t < t1; ++t) {
+        for (int t = from; t < to; ++t) {
             const Half hq = half_of(t + D, qs == 0 ? D : qs - 1, true), hp = half_of(t + D, ps, false);
             piece(std::integral_constant<int, 0>{}, ring + qs * C::QB, ring + RINGP + ps * C::PB, hq);
             mm_wait_dma<(D - 1) * NIQ + (D - 2) * NIP>();            // younger steps may still be on their way
@@ -258,8 +259,17 @@ __global__ __launch_bounds__(MmCfg<CFG>::WAVES * 64, MmCfg<CFG>::PER_SIMD) void 
             piece(std::integral_constant<int, 1>{}, ring + qs * C::QB, ring + RINGP + ps * C::PB, hp);
         }
     };
-    if (kmin == kmax && kmin % BK == 0) run(std::false_type{});
-    else run(std::true_type{});
+    // The first step that holds the end of K.  Steps that fetch only what lies in front of it take the plain loop: chunk by chunk comparisons
+    // cost the training of a block of 3001 x 767 x 2047 219 us against 208.
+    const int cut = t0 < tseg ? tseg - 1 : 2 * tseg - 1, split = kmin == kmax && kmin % BK == 0 ? t1 : cut < t1 ? (cut - D > t0 ? cut - D : t0) : t1;
+    if (split == t1) start(std::false_type{});
+    else start(std::true_type{});
+    mm_wait_dma<(D - 1) * (NIQ + NIP)>();
+    ga_lds_barrier();
+    mm_for<0, NT>([&](auto f) MM_INLINE { read_p(ring + RINGP, std::integral_constant<int, 0>{}, f); });
+    mm_for<0, MT>([&](auto f) MM_INLINE { read_q(ring, std::integral_constant<int, 0>{}, f); });
+    steps(t0, split, std::false_type{});
+    steps(split, t1, std::true_type{});
     mm_wait_dma<0>();
     ga_lds_barrier();                                                // the stages are free: the epilogue turns its tiles there
 
