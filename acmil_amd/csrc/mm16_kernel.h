@@ -7,8 +7,9 @@
 //
 // Layout.  A K step is 64 wide.  Tiles travel global -> LDS by 16-byte LDS-DMA (no registers) through a ring, one barrier a step.  The
 // LDS image is linear in the DMA's lane order, so bank conflicts are avoided by permuting which 16-byte chunk of its row each LANE
-// FETCHES.  K-strided tiles lie in LDS as they lie in memory ([k][row]) and are read by ds_read_b64_tr_b16, which hands every lane four consecutive k of its row: no transposed copy of
-// an operand is ever made.  P feeds the A side of the instruction: a lane then owns 4 consecutive COLUMNS of an output row.
+// FETCHES.  K-strided tiles lie in LDS as they lie in memory ([k][row]) and are read by ds_read_b64_tr_b16, which hands every lane four
+// consecutive k of its row: no transposed copy of an operand is ever made.  P feeds the A side of the instruction: a lane then owns 4
+// consecutive COLUMNS of an output row.
 // The epilogue turns the accumulators through LDS (fp32, 68-float rows: conflict-free both ways) into 8 consecutive columns per
 // lane, so bias, residual, saved values and the result move in 16-byte pieces, 128 bytes a row.
 //
