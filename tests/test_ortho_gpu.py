@@ -73,6 +73,30 @@ def test_small_matrices_of_all_shapes_in_one_call():
     check(ops.orthogonalize(gs[3], steps=9, coeffs=(1.5, -0.5, 0.0)), gs[3], steps=9, coeffs=(1.5, -0.5, 0.0))
 
 
+def test_small_matrices_captured_and_with_bad_values():
+    gs = [gradient(20, 70, torch.float32, seed=1), gradient(128, 96, torch.float32, seed=2)]
+    ops.orthogonalize(gs)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = ops.orthogonalize(gs)
+    for _ in range(3):
+        for g in gs:
+            g.normal_()
+        want = ops.orthogonalize(gs)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(want, held))
+    for bad in (float("nan"), float("inf")):
+        g = gradient(20, 70, torch.float32, seed=1)
+        g[3, 4] = bad
+        o = ops.orthogonalize([g, gs[0]])
+        assert o[0].isnan().all() and torch.equal(o[1], want[0])                                           # a neighbour of the same launch is not touched
+    assert not ops.orthogonalize(torch.zeros(3, 20, 70, device="cuda")).any()
+    one = torch.full((1, 1), -3.0, device="cuda")
+    want, bound = iterate(one, torch.float64)                                                # a single value: fp32 may be off by next to nothing, by chance
+    assert (ops.orthogonalize(one).double() - want).abs() <= bound + 2.0 ** -24              # (the docstring's second bound: 16 * 2^-22 |X| a step, times 3.9)
+
+
 @pytest.mark.parametrize("m, n", [(1500, 1900), (2900, 2700)])
 def test_larger_tiles(m, n):
     g = gradient(m, n, torch.float32)
