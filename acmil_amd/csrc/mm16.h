@@ -12,6 +12,8 @@ enum { MM_ACT = 0, MM_GATE = 1, MM_GATE_BWD = 2, MM_PART = 3 };
 
 enum { MM_S = 0, MM_L = 1, MM_D = 2, MM_R32 = 3, MM_R64 = 4 };   // tile configurations of mm16_kernel.h
 
+constexpr int mm_wave_rows(int cfg) { return cfg == MM_D ? 4 : cfg == MM_R32 || cfg == MM_R64 ? 1 : 2; }     // waves of a tile along its rows
+
 struct MmEpi {
     int act, vec;                      // vec: every row that is touched starts on 16 bytes
     const void *bias, *bias2;          // [N] in the operands' type, or null (bias2: of the second factor)
@@ -22,6 +24,7 @@ struct MmEpi {
     float *pre, *pre2; long long ldp;  // fp32 [M, ldp]: kept pre-activations (written by MM_ACT / MM_GATE, read by MM_GATE_BWD), or null
     float* part;                       // MM_PART: [splits][factors][M][ldpart]
     int ldpart;
+    float* sums;                       // MM_GATE_BWD: null, or [tile rows x waves][2 npad]: column sums of dg and du before they are rounded
 };
 
 struct MmArgs {
@@ -202,7 +205,8 @@ template <bool BF> __device__ __forceinline__ void mm_epi_gate(const MmEpi& e, i
     mm_put8<BF>(e.out, m * e.ldo, n, N, e.npad, true, g);      // h: rows of the library's own buffer, always on 16 bytes
 }
 
-template <bool BF> __device__ __forceinline__ void mm_epi_gate_bwd(const MmEpi& e, int m, int n, int N, float* v) {
+// sg, su: += dg, du as they are before they are rounded (a bias gradient sums them: with rounded ones it is off by half as much again)
+template <bool BF> __device__ __forceinline__ void mm_epi_gate_bwd(const MmEpi& e, int m, int n, int N, float* v, float* sg, float* su) {
     if (n >= e.npad) return;
     float g[8], u[8], a[8], slope[8];
     mm_ldf8(e.pre + m * e.ldp + n, g);
@@ -212,6 +216,8 @@ template <bool BF> __device__ __forceinline__ void mm_epi_gate_bwd(const MmEpi& 
     for (int j = 0; j < 8; ++j) {
         g[j] = v[j] * u[j] * slope[j];
         u[j] = v[j] * a[j];
+        sg[j] += n + j < N ? g[j] : 0.0f;
+        su[j] += n + j < N ? u[j] : 0.0f;
     }
     mm_put8<BF>(e.out, m * e.ldo, n, N, e.npad, true, g);
     mm_put8<BF>(e.out2, m * e.ldo, n, N, e.npad, true, u);

@@ -82,16 +82,8 @@ template <bool BF> __global__ __launch_bounds__(256) void mm_colsum_join_kernel(
     ((typename MmEl<BF>::T*)out)[c] = (typename MmEl<BF>::T)t;
 }
 
-// the K ranges of a split product, added in their order, and its epilogue
-template <bool BF, int EPI>
-__global__ __launch_bounds__(256) void mm_join_kernel(MmArgs a) {
-    const int cpr = a.e.ldpart / 8;
-    const long long total = (long long)a.M * cpr;
-    const long long i = blockIdx.x * 256LL + threadIdx.x;
-    if (i >= total) return;
-    const int m = (int)(i / cpr), n = (int)(i - (long long)m * cpr) * 8;
-    constexpr int NF = EPI == MM_GATE ? 2 : 1;
-    float v[NF][8];
+// the K ranges of a split product, added in their order
+template <int NF> __device__ __forceinline__ void mm_join8(const MmArgs& a, int m, int n, float (*v)[8]) {
 #pragma unroll
     for (int f = 0; f < NF; ++f)
 #pragma unroll
@@ -105,9 +97,44 @@ __global__ __launch_bounds__(256) void mm_join_kernel(MmArgs a) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[f][j] += w[j];
         }
+}
+// ... and the epilogue
+template <bool BF, int EPI>
+__global__ __launch_bounds__(256) void mm_join_kernel(MmArgs a) {
+    const int cpr = a.e.ldpart / 8;
+    const long long total = (long long)a.M * cpr;
+    const long long i = blockIdx.x * 256LL + threadIdx.x;
+    if (i >= total) return;
+    const int m = (int)(i / cpr), n = (int)(i - (long long)m * cpr) * 8;
+    constexpr int NF = EPI == MM_GATE ? 2 : 1;
+    float v[NF][8];
+    mm_join8<NF>(a, m, n, v);
     if constexpr (EPI == MM_GATE) mm_epi_gate<BF>(a.e, m, n, a.N, v[0], v[1]);
-    else if constexpr (EPI == MM_GATE_BWD) mm_epi_gate_bwd<BF>(a.e, m, n, a.N, v[0]);
     else mm_epi_act<BF>(a.e, m, n, a.N, v[0]);
+}
+// ... and the gate's backward, with the column sums (e.sums [gridDim.y][2 npad]): a run of rows of 256 columns a workgroup, 8 rows a time
+template <bool BF> __global__ __launch_bounds__(256) void mm_join_gate_bwd_kernel(MmArgs a) {
+    __shared__ float red[8][32][17];
+    const int cx = threadIdx.x & 31, ry = threadIdx.x >> 5, n = (blockIdx.x * 32 + cx) * 8;
+    const int per = (a.M + gridDim.y - 1) / gridDim.y, r0 = blockIdx.y * per, r1 = r0 + per < a.M ? r0 + per : a.M;
+    float sums[16] = {};
+    if (n < a.e.npad)
+        for (int m = r0 + ry; m < r1; m += 8) {
+            float v[1][8];
+            mm_join8<1>(a, m, n, v);
+            mm_epi_gate_bwd<BF>(a.e, m, n, a.N, v[0], sums, sums + 8);
+        }
+    if (!a.e.sums) return;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) red[ry][cx][j] = sums[j];
+    __syncthreads();
+    for (int i = threadIdx.x; i < 512; i += 256) {                   // factor, column
+        const int f = i >> 8, c = i & 255, col = blockIdx.x * 256 + c;
+        float t = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) t += red[k][c >> 3][8 * f + (c & 7)];
+        if (col < a.e.npad) a.e.sums[(size_t)blockIdx.y * 2 * a.e.npad + f * a.e.npad + col] = t;
+    }
 }
 
 // ------------------------------------------------------------------------------------------------ host
@@ -174,11 +201,20 @@ void aligned_pair(Ctx& c, Mat& a, Mat& b) {
 
 enum { FWD, DGRAD, WGRAD };
 
+// runs of rows of mm_join_gate_bwd_kernel: at least 8 rows each, up to 2048 workgroups
+int join_gate_rows(const MmArgs& a) {
+    const int gx = (a.e.npad + 255) / 256, most = gx >= 256 ? 8 : 2048 / gx, gy = (a.M + 7) / 8;
+    return gy > most ? most : gy;
+}
+
 void join(Ctx& c, const MmArgs& a, int epi) {
     const dim3 g((unsigned)(((long long)a.M * (a.e.ldpart / 8) + 255) / 256));
 #define JOIN(B, E) hipLaunchKernelGGL((mm_join_kernel<B, E>), g, dim3(256), 0, c.st, a)
-    if (epi == MM_GATE) { if (c.bf) JOIN(true, MM_GATE); else JOIN(false, MM_GATE); }
-    else if (epi == MM_GATE_BWD) { if (c.bf) JOIN(true, MM_GATE_BWD); else JOIN(false, MM_GATE_BWD); }
+    if (epi == MM_GATE_BWD) {
+        const dim3 gb((a.e.npad + 255) / 256, join_gate_rows(a));
+        if (c.bf) hipLaunchKernelGGL((mm_join_gate_bwd_kernel<true>), gb, dim3(256), 0, c.st, a);
+        else hipLaunchKernelGGL((mm_join_gate_bwd_kernel<false>), gb, dim3(256), 0, c.st, a);
+    } else if (epi == MM_GATE) { if (c.bf) JOIN(true, MM_GATE); else JOIN(false, MM_GATE); }
     else { if (c.bf) JOIN(true, MM_ACT); else JOIN(false, MM_ACT); }
 #undef JOIN
     c.launched();
@@ -212,8 +248,12 @@ int slim_splits(long long tiles, int steps, int bm, double outputs) {
     return best;
 }
 
-// One product: tile, K split, launch, join.
-void product(Ctx& c, int kind, MmArgs a, int epi) {
+template <bool BF> void colsum_join(Ctx& c, const float* part, int n, int cols8, int cols, void* out) {
+    hipLaunchKernelGGL((mm_colsum_join_kernel<BF>), dim3((cols + 31) / 32), dim3(256), 0, c.st, part, n, cols8, cols, out);
+}
+
+// One product: tile, K split, launch, join.  sums (MM_GATE_BWD): null, or [2 npad] for the column sums of dg and du.
+void product(Ctx& c, int kind, MmArgs a, int epi, void* sums = nullptr) {
     const bool dual = epi == MM_GATE;
     const int n_eff = dual ? 2 * a.N : a.N, steps = mm_steps(a);
     const long long tl = (long long)((a.M + 255) / 256) * ((n_eff + 255) / 256);
@@ -234,12 +274,20 @@ void product(Ctx& c, int kind, MmArgs a, int epi) {
         a.e.ldpart = r8(a.e.npad);
         a.e.part = (float*)c.ar.take((size_t)a.splits * (dual ? 2 : 1) * a.M * a.e.ldpart * 4);
     }
+    const int cfg = large ? MM_L : slim ? (bm == 32 ? MM_R32 : MM_R64) : tiles * a.splits <= 256 ? MM_D : MM_S;
+    const int rows = a.splits > 1 ? join_gate_rows(a) : a.ntm * mm_wave_rows(cfg);
+    if (sums) a.e.sums = (float*)c.ar.take((size_t)rows * 2 * a.e.npad * 4);
     flush(c);
     if (c.room() && c.go()) {
-        const int e = a.splits > 1 ? MM_PART : epi, cfg = large ? MM_L : slim ? (bm == 32 ? MM_R32 : MM_R64) : tiles * a.splits <= 256 ? MM_D : MM_S;
+        const int e = a.splits > 1 ? MM_PART : epi;
         c.rc = kind == FWD ? mm_launch_fwd(a, c.bf, e, dual, cfg, c.st) : kind == DGRAD ? mm_launch_dgrad(a, c.bf, e, cfg, c.st)
                                                                              : mm_launch_wgrad(a, c.bf, e, cfg, c.st);
         if (a.splits > 1 && c.rc == ACMIL_OK) join(c, a, epi);
+        if (sums && c.rc == ACMIL_OK) {
+            if (c.bf) colsum_join<true>(c, a.e.sums, rows, 2 * a.e.npad, 2 * a.e.npad, sums);
+            else colsum_join<false>(c, a.e.sums, rows, 2 * a.e.npad, 2 * a.e.npad, sums);
+            c.launched();
+        }
     }
     c.ar.off = mark;                                                 // the partial sums are dead behind the join: stream order
 }
@@ -275,8 +323,8 @@ void colsum(Ctx& c, const Mat& x, int rows, int cols, void* out, const float* z 
         if (z) { if (c.bf) COLSUM(true, true); else COLSUM(false, true); }
         else { if (c.bf) COLSUM(true, false); else COLSUM(false, false); }
 #undef COLSUM
-        if (part && c.bf) hipLaunchKernelGGL((mm_colsum_join_kernel<true>), dim3((cols + 31) / 32), dim3(256), 0, c.st, part, gy, c8, cols, out);
-        else if (part) hipLaunchKernelGGL((mm_colsum_join_kernel<false>), dim3((cols + 31) / 32), dim3(256), 0, c.st, part, gy, c8, cols, out);
+        if (part && c.bf) colsum_join<true>(c, part, gy, c8, cols, out);
+        else if (part) colsum_join<false>(c, part, gy, c8, cols, out);
         c.launched();
     }
     c.ar.off = mark;
@@ -427,7 +475,7 @@ int ffn_bwd(const acmil_ffn_args& a, Ctx& c) {
         output(p, (void*)dgu.p, 2LL * F8);
         p.e.out2 = (short*)dgu.p + F8; p.e.npad = F8; p.e.act = a.act;
         p.e.pre = a.g; p.e.pre2 = a.u; p.e.ldp = F8;
-        product(c, DGRAD, p, MM_GATE_BWD);
+        product(c, DGRAD, p, MM_GATE_BWD, a.dbgu);
     }
     if (a.dx) {
         MmArgs p = operands(dgu, wg, a.M, a.D, F8, a.F);             // dg Wg + du Wu: two K segments of one product
@@ -446,7 +494,6 @@ int ffn_bwd(const acmil_ffn_args& a, Ctx& c) {
         output(p, a.dWd, a.F);
         product(c, WGRAD, p, MM_ACT);
     }
-    if (a.dbgu) colsum(c, dgu, a.M, 2 * F8, a.dbgu);
     if (a.dbd) colsum(c, dy, a.M, a.D, a.dbd);
     return c.rc;
 }

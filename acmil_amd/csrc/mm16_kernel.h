@@ -281,6 +281,7 @@ __global__ __launch_bounds__(MmCfg<CFG>::WAVES * 64, MmCfg<CFG>::PER_SIMD) void 
     static_assert(C::WAVES * HB * 16 * 68 * 4 <= RINGP + D * C::PB, "room for the turned tiles");
     float* st = (float*)smem + wave * (HB * 16 * 68);
     const int mrow = m0 + wm * C::TM;
+    float sg[8] = {}, su[8] = {};                                    // MM_GATE_BWD: sums over this wave's rows
 #pragma unroll
     for (int i = 0; i < MT / HB; ++i) {
 #pragma unroll
@@ -296,7 +297,7 @@ __global__ __launch_bounds__(MmCfg<CFG>::WAVES * 64, MmCfg<CFG>::PER_SIMD) void 
                 mm_ldf8(st + row * 68 + c, v);
                 if (m < a.M) {
                     if constexpr (EPI == MM_ACT) mm_epi_act<BF>(a.e, m, n, a.N, v);
-                    else if constexpr (EPI == MM_GATE_BWD) mm_epi_gate_bwd<BF>(a.e, m, n, a.N, v);
+                    else if constexpr (EPI == MM_GATE_BWD) mm_epi_gate_bwd<BF>(a.e, m, n, a.N, v, sg, su);
                     else if (n < a.e.ldpart) mm_stf8(a.e.part + ((size_t)blockIdx.y * a.M + m) * a.e.ldpart + n, v);
                 }
             }
@@ -319,9 +320,27 @@ __global__ __launch_bounds__(MmCfg<CFG>::WAVES * 64, MmCfg<CFG>::PER_SIMD) void 
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
+    if constexpr (EPI == MM_GATE_BWD) {
+        const int n = n0 + wn * 64 + (lane & 7) * 8;
+        if (a.e.sums) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+#pragma unroll
+                for (int o = 8; o < 64; o <<= 1) {
+                    sg[j] += __shfl_xor(sg[j], o);
+                    su[j] += __shfl_xor(su[j], o);
+                }
+            if (lane < 8 && n < a.e.npad) {
+                float* to = a.e.sums + (size_t)(tm * (C::BM / C::TM) + wm) * 2 * a.e.npad + n;
+                mm_stf8(to, sg);
+                mm_stf8(to + a.e.npad, su);
+            }
+        }
+    }
 }
 
 template <bool BF, int PK, int QK, int EPI, bool DUAL, int CFG> static inline int mm_go(const MmArgs& a, hipStream_t st) {
+    static_assert(MmCfg<CFG>::BM / MmCfg<CFG>::TM == mm_wave_rows(CFG), "rows of MmEpi::sums");
     hipLaunchKernelGGL((mm16_kernel<BF, PK, QK, EPI, DUAL, CFG>), dim3(a.ntm * a.ntn, a.splits), dim3(MmCfg<CFG>::WAVES * 64), 0, st, a);
     return hipGetLastError() == hipSuccess ? ACMIL_OK : ACMIL_ERR_LAUNCH;
 }

@@ -609,7 +609,7 @@ int acmil_adamw_step_peer(float* params, float* exp_avg, float* exp_avg_sq, long
  *     backward, all three or none (h then lives in the workspace).
  *   acmil_gated_ffn_bwd   dh = dy Wd, dg = dh u act'(g), du = dh act(g) (both held in the tensors' type);
  *     dx = dg Wg + du Wu; dWgu [2 round8(F)][D]: rows 0.. = dg^T x, rows round8(F).. = du^T x; dWd [D,F] = dy^T h;
- *     dbgu [2 round8(F)]: dbg, dbu likewise; dbd [D]  (each may be NULL; dense)
+ *     dbgu [2 round8(F)]: dbg, dbu likewise (sums of dg, du before they are rounded); dbd [D]  (each may be NULL; dense)
  * Results are reproducible bit for bit (no atomics; K splits are joined in a fixed order).
  * workspace: acmil_*_workspace_bytes(args) bytes, 256-byte aligned, contents arbitrary, dead when the call's work is done.  The
  * query reads the same argument block (base addresses included: they decide about copies); 0 = the arguments are refused.
