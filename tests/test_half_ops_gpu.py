@@ -363,6 +363,21 @@ def test_gradients_against_differences():
         assert (slope - (d.double() * e).sum()).abs() <= bound, k
 
 
+@pytest.mark.parametrize("M, D, F", [(4200, 64, 2700), (300, 72, 1000), (90, 2048, 300), (5, 40, 33)])
+def test_ffn_bias_gradients_alone(M, D, F):
+    """256-wide tiles, 128-wide ones, a split K, few rows; asked for alone they are what they are beside everything else, and the padding is zero"""
+    t = make_ffn(M, D, F, torch.float16, seed=5)
+    check_ffn(t, "gelu")
+    y, saved = ops.gated_ffn(t["x"].detach(), t["wg"].detach(), t["wu"].detach(), t["wd"].detach(), keep=True)
+    args = (t["dy"], t["x"].detach(), t["wg"].detach(), t["wu"].detach(), t["wd"].detach(), saved)
+    alone = ops.gated_ffn_bwd(*args, need_x=False, need_gate_up=False, need_down=False, need_gate_up_bias=True)
+    every = ops.gated_ffn_bwd(*args, need_gate_up_bias=True, need_down_bias=True)
+    assert alone[0] is None and alone[1] is None and alone[6] is None
+    assert torch.equal(alone[4], every[4]) and torch.equal(alone[5], every[5])
+    whole = alone[4].as_strided((2 * ((F + 7) // 8 * 8),), (1,), 0)
+    assert not whole[F:(F + 7) // 8 * 8].any() and not whole[(F + 7) // 8 * 8 + F:].any()
+
+
 def test_mixed_needs():
     """only the gradients that are asked for are formed; the others are None"""
     x, w, b, r, dy = make_linear(50, 64, 40, torch.bfloat16)
