@@ -22,10 +22,12 @@ __global__ __launch_bounds__(256) void mm_pad_kernel(MmPads a) {
         const long long q = i - a.m[k].first;
         const int r = (int)(q / cpr), c = (int)(q - (long long)r * cpr) * 8;
         const short* s = a.m[k].src + r * a.m[k].lds + c;
-        short v[8];
+        mm_any8 v;
+        if (c + 8 <= cols) v = *(const mm_any8*)s;
+        else
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = c + j < cols ? s[j] : (short)0;
-        *(uint4*)(a.m[k].dst + (long long)r * ldd + c) = *(const uint4*)v;
+            for (int j = 0; j < 8; ++j) v[j] = c + j < cols ? s[j] : (short)0;
+        *(mm_any8*)(a.m[k].dst + (long long)r * ldd + c) = v;
     }
 }
 
@@ -34,7 +36,7 @@ __global__ __launch_bounds__(256) void mm_pad_kernel(MmPads a) {
 // 8 << lcx columns, 256 >> lcx rows a time.  Sums go to part [gridDim.y][cols8], or straight to out where one workgroup has all rows: two
 // passes of fixed order, no atomics.  Bound by its bytes: 8 a value with dz, 2 without.
 template <bool BF, bool DZ>
-__global__ __launch_bounds__(256) void mm_colsum_kernel(const void* __restrict__ x, long long ld, int vec, int rows, int cols, int cols8, int lcx,
+__global__ __launch_bounds__(256) void mm_colsum_kernel(const void* __restrict__ x, long long ld, int rows, int cols, int cols8, int lcx,
                                                         const float* __restrict__ z, int act, void* __restrict__ dz, float* __restrict__ part,
                                                         void* __restrict__ out) {
     __shared__ float red[256][9];
@@ -46,12 +48,12 @@ __global__ __launch_bounds__(256) void mm_colsum_kernel(const void* __restrict__
             float v[8];
             if constexpr (DZ) {
                 float p[8], a[8], slope[8];
-                mm_row8<BF>(x, r * ld, c, cols, vec != 0, v);
+                mm_row8<BF>(x, r * ld, c, cols, v);
                 mm_ldf8(z + (long long)r * cols8 + c, p);
                 mm_act_slope8(act, p, a, slope);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) v[j] *= slope[j];
-                mm_put8<BF>(dz, (long long)r * cols8, c, cols, cols8, true, v);
+                mm_put8<BF>(dz, (long long)r * cols8, c, cols, cols8, v);
             } else mm_ld8<BF>(x, r * ld + c, v);
 #pragma unroll
             for (int j = 0; j < 8; ++j) s[j] += v[j];
@@ -223,7 +225,7 @@ void join(Ctx& c, const MmArgs& a, int epi) {
 // How many ways to split K of a product of 128 x 128 tiles.  A step of one tile takes about 0.55 us alone on its CU and 1.0 us beside
 // another; a split costs a join launch and 8 bytes of partial sums per output and part, written and read at about 4 TB/s.  The rule without
 // these costs, as many parts as fill 512 workgroups, took 20.2 us for 2000 x 768 x 768 against 11.2, and 19.4 for 64 x 4096 x 4096 against 15.4.
-int mm_splits(long long tiles, int steps, double outputs) {
+int mm_splits(long long tiles, int steps, double outputs, double* cost = nullptr) {
     int best = 1;
     double least = 1e30;
     for (int s = 1; s <= 64 && s * 4 <= (steps > 4 ? steps : 4); ++s) {
@@ -232,6 +234,7 @@ int mm_splits(long long tiles, int steps, double outputs) {
         const double us = ((steps + s - 1) / s) * step + (s > 1 ? 2.5 + s * outputs * 8.0 / 4e6 : 0.0);
         if (us < least) { least = us; best = s; }
     }
+    if (cost) *cost = least;
     return best;
 }
 
@@ -252,14 +255,42 @@ template <bool BF> void colsum_join(Ctx& c, const float* part, int n, int cols8,
     hipLaunchKernelGGL((mm_colsum_join_kernel<BF>), dim3((cols + 31) / 32), dim3(256), 0, c.st, part, n, cols8, cols, out);
 }
 
-// One product: tile, K split, launch, join.  sums (MM_GATE_BWD): null, or [2 npad] for the column sums of dg and du.
-void product(Ctx& c, int kind, MmArgs a, int epi, void* sums = nullptr) {
+// rows from .. from + count - 1 of a product
+MmArgs rows_of(MmArgs a, int kind, int from, int count) {
+    const long long q = kind == WGRAD ? from * 2LL : from * a.ldq, o = from * a.e.ldo * 2;
+    a.q0 += q; a.q1 += q;
+    a.e.out = (char*)a.e.out + o;
+    if (a.e.out2) a.e.out2 = (char*)a.e.out2 + o;
+    if (a.e.res) a.e.res = (const char*)a.e.res + from * a.e.ldr * 2;
+    if (a.e.pre) a.e.pre += from * a.e.ldp;
+    if (a.e.pre2) a.e.pre2 += from * a.e.ldp;
+    a.M = count;
+    return a;
+}
+
+// One product: tile, K split, launch, join.  sums (MM_GATE_BWD): null, or [2 npad] for the column sums of dg and du.  whole: rows stay in one launch.
+void product(Ctx& c, int kind, MmArgs a, int epi, void* sums = nullptr, bool whole = false) {
     const bool dual = epi == MM_GATE;
     const int n_eff = dual ? 2 * a.N : a.N, steps = mm_steps(a);
     const long long tl = (long long)((a.M + 255) / 256) * ((n_eff + 255) / 256);
     // 256 x 256 tiles need half the LDS reads and fetches per flop of 128 x 128 ones, but only one fits a CU: taken where they fill
     // most of the 256 CUs
     const bool large = tl >= 160;
+    if (large && tl > 256 && tl % 256 != 0 && !sums && !whole) {
+        // The last round of large tiles leaves CUs without work.  A full round takes about 10 us and 1.4 us a step; where its rows take less as
+        // a product of their own, by 128 x 128 tiles (6 us for the launch), they become one: 50000 x 1536 x 768 OLDUS us without, NEWUS with.
+        const long long row = (n_eff + 255) / 256, kept = (tl - tl % 256) / row * 256;
+        if (kept > 0 && kept < a.M) {
+            double cost;
+            const int rest = a.M - (int)kept;
+            mm_splits((long long)((rest + 127) / 128) * ((n_eff + 127) / 128), steps, (double)rest * r8(a.e.npad) * (dual ? 2 : 1), &cost);
+            if (cost + 6.0 < 10.0 + 1.4 * steps) {
+                product(c, kind, rows_of(a, kind, 0, (int)kept), epi, nullptr, true);
+                product(c, kind, rows_of(a, kind, (int)kept, rest), epi, nullptr, true);
+                return;
+            }
+        }
+    }
     // up to 64 rows: tiles of as many rows where the weights have to be streamed (below 64 MB the 128-row tiles take 16 us for 64 x 4096 x 4096
     // against 19, and 8.5 for 64 x 1024 x 1024 against 10.3)
     const bool slim = !large && kind != WGRAD && a.M <= 64 && (double)n_eff * steps * 64 >= 33554432.0;
@@ -302,13 +333,12 @@ MmArgs operands(const Mat& q, const Mat& p, int M, int N, int Kq, int Kp) {
 }
 void output(MmArgs& a, void* out, long long ldo, const void* bias = nullptr, const void* res = nullptr, long long ldr = 0) {
     a.e.out = out; a.e.ldo = ldo; a.e.bias = bias; a.e.res = res; a.e.ldr = ldr; a.e.npad = a.N;
-    a.e.vec = on16(out) && ldo % 8 == 0 && on16(bias) && on16(res) && ldr % 8 == 0;      // null is on 16 bytes
 }
 
 // out [cols] = column sums of x (null: none wanted); with z, x is dy and dz [rows][round8(cols)] receives dy act'(z)
 void colsum(Ctx& c, const Mat& x, int rows, int cols, void* out, const float* z = nullptr, int act = ACMIL_ACT_NONE, void* dz = nullptr) {
     const size_t mark = c.ar.off;
-    const int c8 = r8(cols), vec = on16(x.p) && x.ld % 8 == 0;
+    const int c8 = r8(cols);
     int lcx = 0;
     while (lcx < 5 && (8 << lcx) < c8) ++lcx;
     const int gx = (c8 + (8 << lcx) - 1) / (8 << lcx), lanes = 256 >> lcx, most = gx >= 256 ? 8 : 2048 / gx;
@@ -319,7 +349,7 @@ void colsum(Ctx& c, const Mat& x, int rows, int cols, void* out, const float* z 
     flush(c);
     if (c.room() && c.go()) {
         const dim3 g(gx, gy);
-#define COLSUM(B, Z) hipLaunchKernelGGL((mm_colsum_kernel<B, Z>), g, dim3(256), 0, c.st, x.p, x.ld, vec, rows, cols, c8, lcx, z, act, dz, part, out)
+#define COLSUM(B, Z) hipLaunchKernelGGL((mm_colsum_kernel<B, Z>), g, dim3(256), 0, c.st, x.p, x.ld, rows, cols, c8, lcx, z, act, dz, part, out)
         if (z) { if (c.bf) COLSUM(true, true); else COLSUM(false, true); }
         else { if (c.bf) COLSUM(true, false); else COLSUM(false, false); }
 #undef COLSUM
@@ -450,7 +480,6 @@ int ffn_fwd(const acmil_ffn_args& a, Ctx& c) {
     MmArgs p = operands(x, wg, a.M, a.F, few ? a.D : x.cols, few ? a.D : wg.cols);
     p.p1 = (const char*)wu.p;
     output(p, (void*)h.p, F8, a.bg);
-    p.e.vec = p.e.vec && on16(a.bu);
     p.e.bias2 = a.bu; p.e.npad = F8; p.e.act = a.act;
     p.e.pre = a.g; p.e.pre2 = a.u; p.e.ldp = F8;
     if (few) few_rows(c, p, true); else product(c, FWD, p, MM_GATE);

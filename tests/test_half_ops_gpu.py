@@ -66,6 +66,20 @@ def test_linear_large_tiles_and_split_products(M, K, N, dt):
     check_linear(x, w, b, "silu", r, dy)
 
 
+@pytest.mark.parametrize("M, K, N", [(5000, 200, 3500), (4000, 72, 5001), (17000, 136, 1000), (300, 1000, 20000), (5000, 3500, 200)])
+@pytest.mark.parametrize("dt", list(DTS))
+def test_linear_rows_in_two_launches(M, K, N, dt):
+    """more large tiles than CUs, and a last round that is better a product of its own: forward, dx and dW"""
+    x, w, b, r, dy = make_linear(M, K, N, DTS[dt], seed=N)
+    check_linear(x, w, b, "silu", r, dy)
+    check_linear(x.detach(), w.detach(), None, "none", None, dy)
+
+
+@pytest.mark.parametrize("M, D, F", [(5000, 200, 1700), (2600, 3300, 250)])
+def test_ffn_rows_in_two_launches(M, D, F):
+    check_ffn(make_ffn(M, D, F, torch.bfloat16, seed=2), "silu", bias=False)
+
+
 @pytest.mark.parametrize("M, K, N", [(5, 8200, 4100), (20, 4096, 8201), (32, 4104, 8208), (33, 8200, 4104), (64, 4096, 8200)])
 @pytest.mark.parametrize("dt", list(DTS))
 def test_few_rows_by_streamed_weights(M, K, N, dt):
