@@ -277,8 +277,9 @@ void product(Ctx& c, int kind, MmArgs a, int epi, void* sums = nullptr, bool who
     // most of the 256 CUs
     const bool large = tl >= 160;
     if (large && tl > 256 && tl % 256 != 0 && !sums && !whole) {
-        // The last round of large tiles leaves CUs without work.  A full round takes about 10 us and 1.4 us a step; where its rows take less as
-        // a product of their own, by 128 x 128 tiles (6 us for the launch), they become one: 50000 x 1536 x 768 OLDUS us without, NEWUS with.
+        // The last round of large tiles leaves CUs without work.  A full round takes about 10 us and 1.4 us a step; where its rows take less as a
+        // product of their own, by 128 x 128 tiles (6 us for the launch), they become one: 5000 x 2048 x 3500 123 -> 97 us, 10000 x 2048 x 2048
+        // 97 -> 79, 50000 x 1536 x 768 140 -> 135; 7000 x 1024 x 4096, which the rule takes too, 65 -> 66.
         const long long row = (n_eff + 255) / 256, kept = (tl - tl % 256) / row * 256;
         if (kept > 0 && kept < a.M) {
             double cost;
