@@ -1,6 +1,7 @@
 """16-bit linear layer, gated block: what they refuse, on the CPU (nothing reaches a kernel), and the reference's own gradients."""
 import ctypes
 
+import numpy as np
 import pytest
 import torch
 
@@ -121,3 +122,51 @@ def test_muon_entries_and_trainer_option_refuse():
         T.make_optimizer(torch.nn.Linear(64, 64), T.Struct(wd=0.0, optimizer="muon"), torch.device("cpu"))
     with pytest.raises(SystemExit):
         T.get_arguments(["--optimizer", "sgd"])
+
+
+def _largest(a, b, c, u):
+    """the largest |a s + b s^3 + c s^5| and |b s^2 + c s^4| on [0, u], from the roots of their derivatives in 64 bits"""
+    def peak(p):
+        s = [0.0, u] + [r.real for r in p.deriv().roots() if abs(r.imag) < 1e-12 and 0 <= r.real <= u]
+        return max(abs(p(v)) for v in s)
+    P = np.polynomial.Polynomial
+    return peak(P([0, a, 0, b, 0, c])), peak(P([0, 0, b, 0, c]))
+
+
+def test_orthogonalize_coefficients_at_their_limits():
+    """Tables are accepted exactly where the polynomials stay below 3.9 and 15.5.  No workspace is given: an accepted table is refused behind the
+    check (NULL), a refused one by it (SHAPE).  Two tables have a peak beyond the limit between two of 2049 even samples of [0, 1], which stay below."""
+    lib = _lib.load()
+    mats = (_lib.OrthoMat * 1)(_lib.OrthoMat(4096, 16, 4096, 16, 8, 16))
+
+    def accepted(*table):
+        co = (ctypes.c_float * len(table))(*table)
+        rc = lib.acmil_orthogonalize(1, mats, 0, len(table) // 3, co, 1e-7, None, 0, None)
+        assert rc in (-1, -3)
+        return rc == -3
+
+    for between in ((13.233685493469238, -46.426395416259766, 34.76467514038086), (9.997149467468262, -48.42892837524414, 39.40630340576172)):
+        up, bp = _largest(*between, 1.0)
+        s = np.arange(2049) / 2048.0
+        a, b, c = between
+        assert (up > 3.9 or bp > 15.5) and np.abs(a * s + b * s ** 3 + c * s ** 5).max() < 3.9 and np.abs(b * s ** 2 + c * s ** 4).max() < 15.5
+        assert not accepted(*between)
+        assert accepted(*(v * (1 - 1e-5) for v in between))
+    assert accepted(*(ops.NS_COEFFS * 64)) and accepted(1.5, -0.5, 0.0) and accepted(0.0, 0.0, 0.0) and accepted(3.8999, 0.0, 0.0)
+    assert not accepted(3.9001, 0.0, 0.0) and not accepted(0.0, 0.0, 3.9001) and not accepted(float("inf"), 0.0, 0.0)
+    assert not accepted(2.0, 0.0, 0.0, 2.0, 0.0, 0.0) and accepted(2.0, 0.0, 0.0, 1.9, 0.0, 0.0)          # the second step starts where the first ends
+    rng = np.random.default_rng(0)
+    seen = [0, 0]
+    for _ in range(3000):
+        table = np.float32(rng.normal(size=3) * rng.choice([1.0, 4.0, 16.0], 3) * (rng.random(3) < 0.9))
+        table = np.concatenate([table, np.float32(rng.normal(size=3))])
+        u, ok, near = 1.0, True, False
+        for k in (0, 3):
+            up, bp = _largest(*(float(v) for v in table[k:k + 3]), u)
+            near |= abs(up - 3.9) < 1e-6 or abs(bp - 15.5) < 1e-6
+            ok &= up <= 3.9 and bp <= 15.5
+            u = up
+        if not near:
+            assert accepted(*(float(v) for v in table)) == ok, table
+            seen[int(ok)] += 1
+    assert min(seen) > 300
