@@ -1177,6 +1177,7 @@ def _no_overlap(gs, outs) -> None:
 
 
 NS_COEFFS = (3.4445, -4.7750, 2.0315)      # drives singular values from [0.002, 1] into [0.68, 1.14] in 5 steps
+MAX_ORTHO_DIM, MAX_ORTHO_STEPS = 1 << 16, 64
 
 
 def orthogonalize(g, steps: int = 5, coeffs: Sequence = NS_COEFFS, eps: float = 1e-7, out=None):
@@ -1224,7 +1225,7 @@ def orthogonalize(g, steps: int = 5, coeffs: Sequence = NS_COEFFS, eps: float = 
             arr, co = (_lib.OrthoMat * len(mats))(*mats), (ctypes.c_float * len(table))(*table)
             need = lib.acmil_orthogonalize_workspace_bytes(len(mats), arr, _DT[dt])
             if need == 0:
-                raise RuntimeError("acmil_amd.orthogonalize: matrices of at most 65536 rows and columns")
+                raise RuntimeError("acmil_amd.orthogonalize: matrices of at most %d rows and columns" % MAX_ORTHO_DIM)
             ws = torch.empty(need, dtype=torch.uint8, device=dev)
             _lib.check(lib.acmil_orthogonalize(len(mats), arr, _DT[dt], steps, co, float(eps), ws.data_ptr(), need, _stream()), "acmil_orthogonalize")
     return outs if many else outs[0]

@@ -311,17 +311,17 @@ class FlatMuon(FlatAdamW):
     """Orthogonalised momentum for the weight MATRICES, AdamW for everything else, over FlatAdamW's flat buffers:
         buf = mu buf + g;  O = orthogonalize(nesterov ? g + mu buf : buf);  p = p (1 - lr wd) - lr 0.2 sqrt(max(m, n)) O
     (0.2 sqrt(max(m, n)) gives an update the root mean square of AdamW's, so that learning rates and weight decays of AdamW carry over.)
-    A matrix is a 2-D parameter with both sides >= 32: projections and attention branches, not the score row of each branch or the class
-    heads; `muon` = the parameters themselves overrules that.  All matrices share the launches of one acmil_orthogonalize call.
+    A matrix is a 2-D parameter with both sides >= 32 (and at most the 65536 that acmil_orthogonalize takes): projections and attention branches, not
+    the score row of each branch or the class heads; `muon` = the parameters themselves overrules that.  All matrices share the launches of one
+    acmil_orthogonalize call.  0 <= momentum < 1 and 1 <= ns_steps <= 64, looked at again by every step before anything changes.
     The momentum lives in exp_avg.  A raised range flag skips the whole step on the device, as in FlatAdamW.  The update cannot run
     inside the training step's own library call, and there is no direct peer reduction."""
 
     def __init__(self, params: Iterable[torch.nn.Parameter], lr: float = 1e-3, momentum: float = 0.95, nesterov: bool = True, ns_steps: int = 5,
                  betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, grad_buffer: Optional[torch.Tensor] = None,
                  on_step: Optional[Callable[[], None]] = None, muon: Optional[Iterable[torch.nn.Parameter]] = None):
+        self._check_group(momentum, ns_steps)
         super().__init__(params, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, grad_buffer=grad_buffer, on_step=on_step)
-        if not 0.0 <= momentum < 1.0 or ns_steps < 1:
-            raise ValueError("acmil_amd.FlatMuon: 0 <= momentum < 1 and ns_steps >= 1")
         chosen = None if muon is None else {id(p) for p in muon}
         known = {id(p) for p in self.params}
         if chosen is not None and not chosen <= known:
@@ -329,9 +329,10 @@ class FlatMuon(FlatAdamW):
         segs, self._runs, self._muon_indices, off, at, views = [], [], [], 0, 0, []
         for i, p in enumerate(self.params):
             n = p.numel()
-            if id(p) in chosen if chosen is not None else p.dim() == 2 and min(p.shape) >= 32:
-                if p.dim() != 2 or n == 0:
-                    raise RuntimeError("acmil_amd.FlatMuon: only matrices can be orthogonalised, got %s" % (tuple(p.shape),))
+            if id(p) in chosen if chosen is not None else p.dim() == 2 and min(p.shape) >= 32 and max(p.shape) <= ops.MAX_ORTHO_DIM:
+                if p.dim() != 2 or n == 0 or max(p.shape) > ops.MAX_ORTHO_DIM:
+                    raise RuntimeError("acmil_amd.FlatMuon: only matrices of at most %d rows and columns can be orthogonalised, got %s"
+                                       % (ops.MAX_ORTHO_DIM, tuple(p.shape)))
                 segs.append(_lib.MuonSeg(off, n, 0.2 * math.sqrt(max(p.shape))))
                 views.append((at, p.shape))
                 at += n
@@ -349,12 +350,18 @@ class FlatMuon(FlatAdamW):
         self._run_skips = torch.zeros(max(1, len(self._runs)), dtype=torch.int32, device=self.flat.device)      # one counter per AdamW launch
         self.param_groups[0].update(momentum=momentum, nesterov=bool(nesterov), ns_steps=int(ns_steps))
 
+    @staticmethod
+    def _check_group(momentum, ns_steps):
+        if not 0.0 <= momentum < 1.0 or not 1 <= ns_steps <= ops.MAX_ORTHO_STEPS:
+            raise ValueError("acmil_amd.FlatMuon: 0 <= momentum < 1 and 1 <= ns_steps <= %d" % ops.MAX_ORTHO_STEPS)
+
     def can_run_in_step(self) -> bool:
         return False
 
     @torch.no_grad()
     def step(self, track_flag: bool = False) -> int:
         g = self.param_groups[0]
+        self._check_group(g["momentum"], g["ns_steps"])
         track = track_flag and self.guard_flag is not None
         if track and len(self._pending) >= 12:
             raise RuntimeError("acmil_amd.FlatMuon: poll_skipped() must be called while steps are tracked")
@@ -398,6 +405,7 @@ class FlatMuon(FlatAdamW):
         group = sd["param_groups"][0]
         if "muon" in group and list(group["muon"]) != self._muon_indices:
             raise RuntimeError("acmil_amd.FlatMuon: the state's matrices are other parameters than this optimizer's")
+        self._check_group(*(group.get(k, self.param_groups[0][k]) for k in ("momentum", "ns_steps")))
         super().load_state_dict(sd)
         self._run_skips.zero_()
         self.param_groups[0].update({k: group[k] for k in ("momentum", "nesterov", "ns_steps") if k in group})

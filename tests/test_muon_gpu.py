@@ -107,6 +107,52 @@ def test_state_and_choice_of_matrices():
         FlatMuon(parameters(), momentum=1.0)
 
 
+def test_what_a_step_cannot_run_is_refused_before_anything_changes():
+    """more steps than one call takes, a momentum of 1, a matrix of more than 65536 rows: by the constructor, by load_state_dict, and by step() where the
+    group was changed in between -- with parameters, momentum and counters as they were"""
+    for bad in (dict(ns_steps=65), dict(ns_steps=0), dict(momentum=1.0), dict(momentum=-0.1)):
+        with pytest.raises(ValueError):
+            FlatMuon(parameters(), **bad)
+    params = parameters()
+    opt = FlatMuon(params, lr=1e-2)
+    set_grads(params, 0)
+    opt.step()
+
+    def seen():
+        return [opt.flat.clone(), opt.exp_avg.clone(), opt.exp_avg_sq.clone()], (opt.step_count, opt._step_id, opt._launches, opt.mutations)
+
+    tensors, counters = seen()
+    for key, value in (("ns_steps", 65), ("ns_steps", 0), ("momentum", 1.0), ("momentum", float("nan"))):
+        good = opt.param_groups[0][key]
+        opt.param_groups[0][key] = value
+        with pytest.raises(ValueError):
+            opt.step()
+        opt.param_groups[0][key] = good
+        sd = opt.state_dict()
+        sd["param_groups"][0][key] = value
+        with pytest.raises(ValueError):
+            opt.load_state_dict(sd)
+        now, count = seen()
+        assert count == counters and all(torch.equal(a, b) for a, b in zip(now, tensors)) and opt.param_groups[0][key] == good
+    twin = parameters()
+    other = FlatMuon(twin, lr=1e-2)
+    for k in (0, 1):
+        set_grads(twin, k)
+        other.step()
+    set_grads(params, 1)
+    opt.step()
+    assert torch.equal(opt.flat, other.flat)                       # the refusals left no trace
+    tall = torch.nn.Parameter(torch.full((65537, 32), 0.5, device="cuda"))
+    with pytest.raises(RuntimeError, match="at most 65536"):
+        FlatMuon([tall], muon=[tall])
+    rest = torch.nn.Parameter(torch.full((40, 32), 0.5, device="cuda"))
+    opt = FlatMuon([tall, rest], lr=1e-2, weight_decay=0.0)        # left to AdamW: the first step moves every value by lr
+    assert opt._muon_indices == [1]
+    opt.grad[:-1].fill_(1.0)                                       # (the last slot is the range flag)
+    opt.step()
+    assert ((tall - 0.49).abs() <= 1e-6).all()                     # 0.5 - 1e-2 / (1 + 1e-8), three roundings of values below 1
+
+
 def test_more_matrices_than_one_launch_holds():
     g = torch.Generator().manual_seed(0)
     params = [torch.nn.Parameter((torch.randn(32, 32 + k % 3, generator=g) * 0.1).cuda()) for k in range(70)]
