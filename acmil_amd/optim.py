@@ -360,6 +360,10 @@ class FlatMuon(FlatAdamW):
 
     @torch.no_grad()
     def step(self, track_flag: bool = False) -> int:
+        with torch.cuda.device(self.flat.device):                     # the entries launch on the current device
+            return self._step(track_flag)
+
+    def _step(self, track_flag: bool) -> int:
         g = self.param_groups[0]
         self._check_group(g["momentum"], g["ns_steps"])
         track = track_flag and self.guard_flag is not None

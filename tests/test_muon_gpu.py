@@ -153,6 +153,40 @@ def test_what_a_step_cannot_run_is_refused_before_anything_changes():
     assert ((tall - 0.49).abs() <= 1e-6).all()                     # 0.5 - 1e-2 / (1 + 1e-8), three roundings of values below 1
 
 
+def test_a_step_makes_its_parameters_device_the_current_one(monkeypatch):
+    """every library call of a step is made while the parameters' device is entered, whatever device was current (seen here by what is entered: one
+    device is enough)"""
+    from acmil_amd import _lib, optim
+    params = parameters()
+    opt = FlatMuon(params, lr=1e-2)
+    set_grads(params, 0)
+    inside, calls, real = [], [], _lib.load()
+
+    class Guard(torch.cuda.device):
+        def __init__(self, device):
+            super().__init__(device)
+            self.asked = device
+
+        def __enter__(self):
+            inside.append(self.asked)
+            return super().__enter__()
+
+        def __exit__(self, *e):
+            inside.pop()
+            return super().__exit__(*e)
+
+    class Lib:
+        def __getattr__(self, name):
+            calls.append((name, list(inside)))
+            return getattr(real, name)
+
+    monkeypatch.setattr(torch.cuda, "device", Guard)
+    monkeypatch.setattr(optim._lib, "load", Lib)
+    opt.step()
+    assert {n for n, _ in calls} >= {"acmil_muon_momentum", "acmil_orthogonalize", "acmil_muon_apply", "acmil_adamw_step"}
+    assert all(devices and devices[0] == opt.flat.device for _, devices in calls) and not inside
+
+
 def test_more_matrices_than_one_launch_holds():
     g = torch.Generator().manual_seed(0)
     params = [torch.nn.Parameter((torch.randn(32, 32 + k % 3, generator=g) * 0.1).cuda()) for k in range(70)]
