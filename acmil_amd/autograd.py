@@ -26,6 +26,7 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib, ops
 
@@ -336,6 +337,12 @@ def _no_second(backward):
     return staticmethod(lambda ctx, dy: once(ctx, dy) if torch.is_grad_enabled() else backward(ctx, dy))
 
 
+def _no_tangents(name, *tensors):
+    """Forward-mode derivatives are refused: with gradients off no Function sees the dual tensors, and their tangents would be lost without a word."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("acmil_amd.%s: no forward-mode derivative" % name)
+
+
 class _LinearAct(torch.autograd.Function):
     """acmil_linear_act / _bwd.  Kept for the backward: x, the weight and (for an activation) the pre-activations in FP32 -- a 16-bit copy
     would add a rounding of act'(z) to the one of dz that the gradients already carry."""
@@ -358,8 +365,9 @@ class _LinearAct(torch.autograd.Function):
 
 
 def linear_act(x, weight, bias=None, act="none", residual=None):
-    """Differentiable ops.linear_act: act(x @ weight^T + bias) + residual for fp16 / bf16 tensors (no double backward, no autocast: the
-    tensors are taken as they are)."""
+    """Differentiable ops.linear_act: act(x @ weight^T + bias) + residual for fp16 / bf16 tensors (no double backward, no forward mode, no autocast:
+    the tensors are taken as they are)."""
+    _no_tangents("linear_act", x, weight, bias, residual)
     if not torch.is_grad_enabled():
         return ops.linear_act(x, weight, bias=bias, act=act, residual=residual)
     return _LinearAct.apply(x, weight, bias, residual, act)
@@ -390,7 +398,8 @@ class _GatedFfn(torch.autograd.Function):
 
 def gated_ffn(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None, act="silu", residual=None):
     """Differentiable ops.gated_ffn: (act(x @ w_gate^T + b_gate) * (x @ w_up^T + b_up)) @ w_down^T + b_down + residual for fp16 / bf16
-    tensors (no double backward, no autocast: the tensors are taken as they are)."""
+    tensors (no double backward, no forward mode, no autocast: the tensors are taken as they are)."""
+    _no_tangents("gated_ffn", x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual)
     if not torch.is_grad_enabled():
         return ops.gated_ffn(x, w_gate, w_up, w_down, b_gate=b_gate, b_up=b_up, b_down=b_down, act=act, residual=residual)
     return _GatedFfn.apply(x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual, act)

@@ -170,3 +170,20 @@ def test_orthogonalize_coefficients_at_their_limits():
             assert accepted(*(float(v) for v in table)) == ok, table
             seen[int(ok)] += 1
     assert min(seen) > 300
+
+
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_derivatives_are_refused(grad):
+    """no_grad does not switch forward mode off: a dual tensor in any place raises, and none is left unnoticed; without one the call goes on (to the
+    refusal of CPU tensors)"""
+    dt = torch.float16
+    lin = dict(x=torch.zeros(4, 16, dtype=dt), weight=torch.zeros(16, 16, dtype=dt), bias=torch.zeros(16, dtype=dt), residual=torch.zeros(4, 16, dtype=dt))
+    ffn = dict(x=torch.zeros(4, 16, dtype=dt), w_gate=torch.zeros(16, 16, dtype=dt), w_up=torch.zeros(16, 16, dtype=dt), w_down=torch.zeros(16, 16, dtype=dt),
+               b_gate=torch.zeros(16, dtype=dt), b_up=torch.zeros(16, dtype=dt), b_down=torch.zeros(16, dtype=dt), residual=torch.zeros(4, 16, dtype=dt))
+    with torch.set_grad_enabled(grad), torch.autograd.forward_ad.dual_level():
+        for call, args in ((autograd.linear_act, lin), (autograd.gated_ffn, ffn)):
+            for k, v in args.items():
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    call(**{**args, k: torch.autograd.forward_ad.make_dual(v, torch.ones_like(v))})
+            with pytest.raises(RuntimeError, match="no CPU fallback"):
+                call(**args)
