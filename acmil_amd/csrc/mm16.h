@@ -100,7 +100,8 @@ __device__ __forceinline__ float mm_act_slope(int act, float z, float& slope) {
         }
         case ACMIL_ACT_GELU_TANH: {
             const float s = mm_sigmoid(1.5957691216057308f * (z + 0.044715f * z * z * z));
-            slope = s + z * s * (1.0f - s) * 1.5957691216057308f * (1.0f + 0.134145f * z * z);
+            // (z^2 kept finite: beyond 5e19, which bf16 holds, 0.134145 z z is not, and the 0 in front of it would become NaN)
+            slope = s + z * s * (1.0f - s) * 1.5957691216057308f * (1.0f + 0.134145f * fminf(z * z, 1e30f));
             return z * s;
         }
         case ACMIL_ACT_SIGMOID: { const float s = mm_sigmoid(z); slope = s * (1.0f - s); return s; }

@@ -429,3 +429,22 @@ def test_a_residual_block_trains():
     assert (y.double() - z).norm() <= 16 * 2 ** -8 * z.norm()
     for k, a, b in zip(p, got, want):
         assert (a.double() - b).norm() <= 16 * 2 ** -8 * b.norm(), k
+
+
+@pytest.mark.parametrize("act", ACTS)
+def test_far_values_have_the_slopes_of_their_sides(act):
+    """single features whose pre-activations are as large as bf16 holds: outputs and gradients are those of the 64-bit form (all finite)"""
+    v = [1e15, 1e19, 2e19, 1e20, 1e30, 3e38]
+    x = torch.tensor([s * a for a in v for s in (1, -1)], dtype=torch.bfloat16, device="cuda")[:, None]
+    one = torch.ones(1, 1, dtype=torch.bfloat16, device="cuda")
+    for M in (3, len(x)):
+        out = run_linear(x[:M].clone(), one.clone(), None, act, None, torch.ones(M, 1, dtype=torch.bfloat16, device="cuda"))
+        a, slope = R.act64(act, x[:M].double())
+        assert ((out["y"].double() - a).abs() <= 2.0 ** -8 * a.abs() + 1e-30).all()
+        assert ((out["dx"].double() - slope).abs() <= 2.0 ** -8 * slope.abs() + 1e-30).all()
+    t = {"x": x, "wg": one, "wu": torch.zeros_like(one), "wd": one}
+    t = {k: w.clone().requires_grad_() for k, w in t.items()}
+    y = autograd.gated_ffn(t["x"], t["wg"], t["wu"], t["wd"], b_up=torch.ones(1, dtype=torch.bfloat16, device="cuda"), act=act)       # y = act(x)
+    (dx,) = torch.autograd.grad(y, t["x"], torch.ones_like(y))
+    a, slope = R.act64(act, x.double())
+    assert ((y.double() - a).abs() <= 2.0 ** -7 * a.abs() + 1e-30).all() and ((dx.double() - slope).abs() <= 2.0 ** -7 * slope.abs() + 1e-30).all()
