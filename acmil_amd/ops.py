@@ -1184,7 +1184,8 @@ def orthogonalize(g, steps: int = 5, coeffs: Sequence = NS_COEFFS, eps: float = 
     """acmil_orthogonalize: the Newton-Schulz approximation of the orthogonal factor of each matrix (U V^T of G = U S V^T): X = G / (|G|_F + eps),
     then `steps` times X <- a X + (b A + c A A) X with A = X X^T, on the transpose where a matrix is tall.
     g: [m, n], a stack [..., m, n], or a list of [m, n] of any shapes (one type and device): all matrices share the launches.  fp32, fp16 or bf16,
-    returned in the same type and structure; values are held to 22 bits inside whatever the type.  coeffs: one (a, b, c) or one per step.
+    returned in the same type and structure; inside, whatever the type, values are held to 2^-22 of themselves and 2^-37 of |G|_F.  coeffs: one
+    (a, b, c) or one per step.
     out: contiguous tensor(s) of g's structure, type and shapes to write to; a matrix may be its own output, other overlaps are refused."""
     lib = _lib.load()
     many = isinstance(g, (list, tuple))

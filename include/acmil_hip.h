@@ -667,7 +667,9 @@ int acmil_gated_ffn_bwd(const acmil_ffn_args* args, void* workspace, size_t work
  * count matrices of one dtype (F32 / F16 / BF16) share the launches.  mats: HOST array; g [m,n] and o [m,n] row-major with leading
  * dimensions ldg, ldo >= n (elements); o may be g.  1 <= m, n <= 65536.  coeffs: HOST array [steps][3], 1 <= steps <= 64; refused
  * (ACMIL_ERR_SHAPE) unless the polynomials keep singular values that start in [0, 1] below 3.9 and |b s^2 + c s^4| below 15.5.
- * Values are held as f16 pairs (22 bits) and products accumulate in fp32, whatever the type of g; the norm is formed in 64 bits.
+ * Values are held as f16 pairs and products accumulate in fp32, whatever the type of g; the norm is formed in 64 bits.  A stored value is off by
+ * at most 2^-22 of itself and 2^-37 of |G|_F, which a step multiplies by up to a: less than an fp32 iteration keeps where a matrix holds
+ * values of very different size.
  * A zero matrix gives zeros (eps > 0); infinities or NaN in g give NaN.  Reproducible bit for bit.
  * workspace: acmil_orthogonalize_workspace_bytes(...) (0 = refused), 256-byte aligned, contents arbitrary.
  * ------------------------------------------------------------------------------------------- */
