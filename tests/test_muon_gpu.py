@@ -261,3 +261,19 @@ def test_trainer_runs_with_muon(n_token, bags):
     for n, p in model.named_parameters():
         assert torch.isfinite(p).all()
         assert torch.equal(p, before[n]) == (n_token == 1 and n.startswith("classifier.0")), n
+
+
+def test_two_ranks_on_one_bucket():
+    """data-parallel training with FlatMuon: the direct reducer is closed, a flag of one rank skips the step on both, both ranks and a single process on
+    the averaged gradients agree bit for bit (tests/dist_worker_muon.py)"""
+    import os
+    import socket
+    import subprocess
+    import sys
+    s = socket.socket(); s.bind(("127.0.0.1", 0)); port = s.getsockname()[1]; s.close()
+    env = dict(os.environ)
+    env.setdefault("HSA_ENABLE_IPC_MODE_LEGACY", "0")
+    worker = os.path.join(os.path.dirname(os.path.abspath(__file__)), "dist_worker_muon.py")
+    r = subprocess.run([sys.executable, "-m", "torch.distributed.run", "--nnodes=1", "--nproc-per-node", "2", "--master-addr", "127.0.0.1",
+                        "--master-port", str(port), worker], env=env, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, timeout=100)
+    assert r.returncode == 0 and "MUON_OK" in r.stdout, r.stdout[-3000:]
