@@ -32,7 +32,7 @@ struct NsArgs {
     int count, flip, last;        // flip: XT1 is the present transpose; last: X goes to o
     float a, b, c;
     float eps;
-    const double* part; int nparts;
+    const double* part;
     int first[NS_GROUP + 1];      // first workgroup of each matrix
     NsMat m[NS_GROUP];
 };

@@ -1031,8 +1031,9 @@ def _linear_args(name: str, x: torch.Tensor, weight: torch.Tensor, act: str):
 
 def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, act: str = "none",
                residual: Optional[torch.Tensor] = None, keep_pre: bool = False):
-    """acmil_linear_act: y = act(x @ weight^T + bias) + residual in ONE launch of the product (fp16 or bf16; fp32 accumulation and
-    epilogue, one rounding at the end).  x [..., in], weight [out, in], bias [out], residual [..., out]; act one of none, relu, silu, gelu,
+    """acmil_linear_act: y = act(x @ weight^T + bias) + residual, fp16 or bf16 (fp32 accumulation and epilogue, one rounding at the end).  Bias,
+    activation and residual take no pass over the output of their own; sizes and alignment decide whether there are launches beside the
+    product's (a copy of operands that do not lie on 16 bytes, a split K with its join, the last rows as a product of their own).  x [..., in], weight [out, in], bias [out], residual [..., out]; act one of none, relu, silu, gelu,
     gelu_tanh, sigmoid.  Any row strides and sizes; no rows give an empty result.  keep_pre: also x @ weight^T + bias in fp32
     ([rows, round8(out)]), what linear_act_bwd wants.  No gradient is recorded (acmil_amd.autograd.linear_act is the differentiable form)."""
     dev = _half_inputs("linear_act", x, weight, bias, residual)
@@ -1099,8 +1100,8 @@ def _ffn_args(name: str, x, w_gate, w_up, w_down, act: str):
 def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, b_gate: Optional[torch.Tensor] = None,
               b_up: Optional[torch.Tensor] = None, b_down: Optional[torch.Tensor] = None, act: str = "silu",
               residual: Optional[torch.Tensor] = None, keep: bool = False):
-    """acmil_gated_ffn: y = (act(x @ w_gate^T + b_gate) * (x @ w_up^T + b_up)) @ w_down^T + b_down + residual, fp16 or bf16, two launches:
-    both projections, the activation and the product in one, the projection back with bias and residual in the other.  x [..., D], w_gate and
+    """acmil_gated_ffn: y = (act(x @ w_gate^T + b_gate) * (x @ w_up^T + b_up)) @ w_down^T + b_down + residual, fp16 or bf16, in two products:
+    both projections with the activation and the gate, then the projection back with bias and residual (launches beside them as in linear_act).  x [..., D], w_gate and
     w_up [F, D], w_down [D, F], residual [..., D]; act as linear_act ("silu" is the SwiGLU block, "gelu" GeGLU, "sigmoid" GLU, ...).
     The gated features between the launches are held in x's type (in fp16, beyond 65504 they are infinite).  keep: also (g, u, h) for
     gated_ffn_bwd (g, u fp32 and h, each [rows, round8(F)]).  No gradient is recorded (acmil_amd.autograd.gated_ffn is the differentiable form)."""
