@@ -448,3 +448,27 @@ def test_far_values_have_the_slopes_of_their_sides(act):
     (dx,) = torch.autograd.grad(y, t["x"], torch.ones_like(y))
     a, slope = R.act64(act, x.double())
     assert ((y.double() - a).abs() <= 2.0 ** -7 * a.abs() + 1e-30).all() and ((dx.double() - slope).abs() <= 2.0 ** -7 * slope.abs() + 1e-30).all()
+
+
+@pytest.mark.parametrize("M", [2, 20, 70, 300])
+def test_subnormal_values_count(M):
+    """fp16 values below 2^-14, as inputs, weights, incoming gradients and results: sums of exact products by powers of two, so every
+    sum is exact (a multiple of 2^-24 below 2^-12) and rounded once"""
+    g = torch.Generator(device="cuda").manual_seed(M)
+
+    def small(*shape):
+        return (torch.randint(-1023, 1024, shape, generator=g, device="cuda").double() * 2.0 ** -24).half()
+
+    def powers(*shape):
+        return torch.where(torch.randint(0, 2, shape, generator=g, device="cuda") > 0, 1.0, -1.0).half()
+
+    for x, w, dy in ((small(M, 72), powers(40, 72), powers(M, 40)), (powers(M, 72), small(40, 72), small(M, 40))):
+        x[:, 3:] = 0                                                   # three products a sum
+        y = ops.linear_act(x, w)
+        exact = x.double() @ w.double().t()
+        assert torch.equal(y, exact.half()) and bool((exact != 0).any()) and float(exact.abs().max()) < 2.0 ** -12
+        dy[4:] = 0
+        dy[:, 4:] = 0                                                  # dx: four products a sum; dW, db: as many rows
+        dx, dw, db = ops.linear_act_bwd(dy, x, w)
+        assert torch.equal(dx, (dy.double() @ w.double()).half()) and torch.equal(dw, (dy.double().t() @ x.double()).half())
+        assert torch.equal(db, dy.double().sum(0).half())
