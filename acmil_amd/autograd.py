@@ -366,7 +366,7 @@ class _LinearAct(torch.autograd.Function):
 
 def linear_act(x, weight, bias=None, act="none", residual=None):
     """Differentiable ops.linear_act: act(x @ weight^T + bias) + residual for fp16 / bf16 tensors (no double backward, no forward mode, no autocast:
-    the tensors are taken as they are)."""
+    the tensors are taken as they are).  In fp16, gradients of the pre-activations beyond 65504 are infinite."""
     _no_tangents("linear_act", x, weight, bias, residual)
     if not torch.is_grad_enabled():
         return ops.linear_act(x, weight, bias=bias, act=act, residual=residual)
@@ -398,7 +398,9 @@ class _GatedFfn(torch.autograd.Function):
 
 def gated_ffn(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None, act="silu", residual=None):
     """Differentiable ops.gated_ffn: (act(x @ w_gate^T + b_gate) * (x @ w_up^T + b_up)) @ w_down^T + b_down + residual for fp16 / bf16
-    tensors (no double backward, no forward mode, no autocast: the tensors are taken as they are)."""
+    tensors (no double backward, no forward mode, no autocast: the tensors are taken as they are).  In fp16, gated features and gradients of the
+    pre-activations beyond 65504 are infinite.  The gradients of w_gate and w_up, and those of b_gate and b_up, share one storage, and are formed
+    together where one of the two is asked for."""
     _no_tangents("gated_ffn", x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual)
     if not torch.is_grad_enabled():
         return ops.gated_ffn(x, w_gate, w_up, w_down, b_gate=b_gate, b_up=b_up, b_down=b_down, act=act, residual=residual)

@@ -60,7 +60,7 @@ template <> struct MmEl<false> { typedef _Float16 T; typedef f16x8 V; };
 __device__ __forceinline__ float mm_sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + __expf(-z)); }
 
 // Normal distribution function, e = exp(-z^2 / 2).  Phi(-x) = e P(t), t = 1 / (1 + 0.3 x): the form of Abramowitz and Stegun 7.1.26 with a
-// degree-8 P fitted to least relative error over 0 <= x <= 14 (1.5e-7; in fp32: 6e-7 for x < 3, absolute 7e-8, and no loss in the lower tail).
+// degree-8 P fitted to least relative error over 0 <= x <= 14 (1.7e-7; in fp32: 6e-7 for x < 3, absolute 7e-8, and no loss in the lower tail).
 __device__ __forceinline__ float mm_normal_cdf(float z, float& e) {
     const float t = __builtin_amdgcn_rcpf(fmaf(0.3f, fabsf(z), 1.0f));
     float p = 0.03567476198f;

@@ -1061,7 +1061,8 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
 def linear_act_bwd(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, pre: Optional[torch.Tensor] = None, act: str = "none",
                    need: Sequence[bool] = (True, True, True)):
     """acmil_linear_act_bwd: (dx, dweight, dbias) of linear_act for the incoming dy [..., out] and the kept `pre` (act "none" needs none);
-    need = which of the three to form (None in the others' places).  The residual's gradient is dy."""
+    need = which of the three to form (None in the others' places).  dz = dy act'(pre) is held in the tensors' type between the passes (in fp16, beyond
+    65504 it is infinite and below 2^-25 zero: scale the loss accordingly).  The residual's gradient is dy."""
     dev = _half_inputs("linear_act_bwd", x, weight, dy)
     a, x2, w2 = _linear_args("linear_act_bwd", x, weight, act)
     if tuple(dy.shape) != tuple(x.shape[:-1]) + (a.N,):
@@ -1132,7 +1133,8 @@ def gated_ffn_bwd(dy: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w_up:
                   act: str = "silu", need_x: bool = True, need_gate_up: bool = True, need_down: bool = True, need_gate_up_bias: bool = False,
                   need_down_bias: bool = False):
     """acmil_gated_ffn_bwd: (dx, dw_gate, dw_up, dw_down, db_gate, db_up, db_down) of gated_ffn for the incoming dy [..., D] and what
-    gated_ffn(keep=True) kept; None where not asked for.  dw_gate / dw_up and db_gate / db_up are views of one buffer each.  The residual's gradient is dy."""
+    gated_ffn(keep=True) kept; None where not asked for.  dw_gate / dw_up and db_gate / db_up are views of one buffer each.  The gradients of both
+    projections are held in the tensors' type between the products (in fp16, beyond 65504 infinite and below 2^-25 zero).  The residual's gradient is dy."""
     dev = _half_inputs("gated_ffn_bwd", x, w_gate, w_up, w_down, dy)
     a, hold = _ffn_args("gated_ffn_bwd", x, w_gate, w_up, w_down, act)
     if dy.shape != x.shape:
@@ -1186,7 +1188,7 @@ def orthogonalize(g, steps: int = 5, coeffs: Sequence = NS_COEFFS, eps: float = 
     then `steps` times X <- a X + (b A + c A A) X with A = X X^T, on the transpose where a matrix is tall.
     g: [m, n], a stack [..., m, n], or a list of [m, n] of any shapes (one type and device): all matrices share the launches.  fp32, fp16 or bf16,
     returned in the same type and structure; inside, whatever the type, values are held to 2^-22 of themselves and 2^-37 of |G|_F.  coeffs: one
-    (a, b, c) or one per step.
+    (a, b, c) or one per step.  The same list gives the same bits; beside other matrices one may differ in its last.  No gradient is recorded.
     out: contiguous tensor(s) of g's structure, type and shapes to write to; a matrix may be its own output, other overlaps are refused."""
     lib = _lib.load()
     many = isinstance(g, (list, tuple))
