@@ -276,6 +276,7 @@ void product(Ctx& c, int kind, MmArgs a, int epi, void* sums = nullptr, bool who
     // 256 x 256 tiles need half the LDS reads and fetches per flop of 128 x 128 ones, but only one fits a CU: taken where they fill
     // most of the 256 CUs
     const bool large = tl >= 160;
+    // (Not where column sums are formed on the way, the gated block's backward with bias gradients: they are laid out by the row tiles of one launch.)
     if (large && tl > 256 && tl % 256 != 0 && !sums && !whole) {
         // The last round of large tiles leaves CUs without work.  A full round takes about 10 us and 1.4 us a step; where its rows take less as a
         // product of their own, by 128 x 128 tiles (6 us for the launch), they become one: 5000 x 2048 x 3500 123 -> 97 us, 10000 x 2048 x 2048
