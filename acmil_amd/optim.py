@@ -352,8 +352,8 @@ class FlatMuon(FlatAdamW):
 
     @staticmethod
     def _check_group(momentum, ns_steps):
-        if not 0.0 <= momentum < 1.0 or not 1 <= ns_steps <= ops.MAX_ORTHO_STEPS:
-            raise ValueError("acmil_amd.FlatMuon: 0 <= momentum < 1 and 1 <= ns_steps <= %d" % ops.MAX_ORTHO_STEPS)
+        if not 0.0 <= momentum < 1.0 or not 1 <= ns_steps <= ops.MAX_ORTHO_STEPS or ns_steps != int(ns_steps):
+            raise ValueError("acmil_amd.FlatMuon: 0 <= momentum < 1 and a whole number of ns_steps from 1 to %d" % ops.MAX_ORTHO_STEPS)
 
     def can_run_in_step(self) -> bool:
         return False
@@ -366,6 +366,8 @@ class FlatMuon(FlatAdamW):
     def _step(self, track_flag: bool) -> int:
         g = self.param_groups[0]
         self._check_group(g["momentum"], g["ns_steps"])
+        mu, nesterov, steps = float(g["momentum"]), int(g["nesterov"]), int(g["ns_steps"])         # the whole group is read before anything changes
+        lr, wd, eps, b1, b2 = (float(v) for v in (g["lr"], g["weight_decay"], g["eps"], *g["betas"]))
         track = track_flag and self.guard_flag is not None
         if track and len(self._pending) >= 12:
             raise RuntimeError("acmil_amd.FlatMuon: poll_skipped() must be called while steps are tracked")
@@ -373,20 +375,20 @@ class FlatMuon(FlatAdamW):
         self._step_id += 1
         self._launches += 1
         slot = self._step_id % 16
-        lib, b1, b2 = _lib.load(), *g["betas"]
+        lib = _lib.load()
         kept = [(o, self.flat[o:o + n].clone()) for o, n in self._frozen]
         flag = None if self.guard_flag is None else self.guard_flag.data_ptr()
         stream = torch.cuda.current_stream().cuda_stream
         _lib.check(lib.acmil_muon_momentum(len(self._segs), self._segs, self.grad.data_ptr(), self.exp_avg.data_ptr(), self._update.data_ptr(),
-                                           float(g["momentum"]), int(g["nesterov"]), flag, self._host_flags.data_ptr() + 4 * slot if track else None,
+                                           mu, nesterov, flag, self._host_flags.data_ptr() + 4 * slot if track else None,
                                            stream), "acmil_muon_momentum")
-        ops.orthogonalize(self._update_views, steps=g["ns_steps"], out=self._update_views)
-        _lib.check(lib.acmil_muon_apply(len(self._segs), self._segs, self.flat.data_ptr(), self._update.data_ptr(), float(g["lr"]),
-                                        float(g["weight_decay"]), flag, stream), "acmil_muon_apply")
+        ops.orthogonalize(self._update_views, steps=steps, out=self._update_views)
+        _lib.check(lib.acmil_muon_apply(len(self._segs), self._segs, self.flat.data_ptr(), self._update.data_ptr(), lr, wd, flag,
+                                        stream), "acmil_muon_apply")
         for i, (a, b) in enumerate(self._runs):
             _lib.check(lib.acmil_adamw_step(self.flat.data_ptr() + 4 * a, self.grad.data_ptr() + 4 * a, self.exp_avg.data_ptr() + 4 * a,
-                                            self.exp_avg_sq.data_ptr() + 4 * a, b - a, float(g["lr"]), float(b1), float(b2), float(g["eps"]),
-                                            float(g["weight_decay"]), self._launches, flag, self._run_skips.data_ptr() + 4 * i, stream), "acmil_adamw_step")
+                                            self.exp_avg_sq.data_ptr() + 4 * a, b - a, lr, b1, b2, eps, wd, self._launches, flag,
+                                            self._run_skips.data_ptr() + 4 * i, stream), "acmil_adamw_step")
         for o, v in kept:
             self.flat[o:o + v.numel()].copy_(v)
         self.mutations += 1

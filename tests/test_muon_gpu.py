@@ -153,6 +153,26 @@ def test_what_a_step_cannot_run_is_refused_before_anything_changes():
     assert ((tall - 0.49).abs() <= 1e-6).all()                     # 0.5 - 1e-2 / (1 + 1e-8), three roundings of values below 1
 
 
+def test_a_group_that_cannot_be_read_changes_nothing():
+    """a value of the wrong kind in the group raises before the momentum moves: the step can be taken again with a right one"""
+    params = parameters()
+    opt = FlatMuon(params, lr=1e-2)
+    set_grads(params, 0)
+    flat = opt.flat.clone()
+    for key, value in (("ns_steps", 2.5), ("lr", None), ("weight_decay", "much"), ("betas", (0.9, None)), ("nesterov", None)):
+        good = opt.param_groups[0][key]
+        opt.param_groups[0][key] = value
+        with pytest.raises((TypeError, ValueError)):
+            opt.step()
+        opt.param_groups[0][key] = good
+        assert not opt.exp_avg.any() and torch.equal(opt.flat, flat) and opt.step_count == 0 and opt._launches == 0, key
+    twin = parameters()
+    other = FlatMuon(twin, lr=1e-2)
+    set_grads(twin, 0)
+    other.step(), opt.step()
+    assert torch.equal(opt.flat, other.flat)
+
+
 def test_a_step_makes_its_parameters_device_the_current_one(monkeypatch):
     """every library call of a step is made while the parameters' device is entered, whatever device was current (seen here by what is entered: one
     device is enough)"""
