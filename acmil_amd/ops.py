@@ -1033,8 +1033,8 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
                residual: Optional[torch.Tensor] = None, keep_pre: bool = False):
     """acmil_linear_act: y = act(x @ weight^T + bias) + residual, fp16 or bf16 (fp32 accumulation and epilogue, one rounding at the end).  Bias,
     activation and residual take no pass over the output of their own; sizes and alignment decide whether there are launches beside the
-    product's (a copy of operands that do not lie on 16 bytes, a split K with its join, the last rows as a product of their own).  x [..., in], weight [out, in], bias [out], residual [..., out]; act one of none, relu, silu, gelu,
-    gelu_tanh, sigmoid.  Any row strides and sizes; no rows give an empty result.  keep_pre: also x @ weight^T + bias in fp32
+    product's (a copy of operands that do not lie on 16 bytes, a split K with its join, the last rows as a product of their own).
+    x [..., in], weight [out, in], bias [out], residual [..., out]; act one of none, relu, silu, gelu, gelu_tanh, sigmoid.  Any row strides and sizes; no rows give an empty result.  keep_pre: also x @ weight^T + bias in fp32
     ([rows, round8(out)]), what linear_act_bwd wants.  No gradient is recorded (acmil_amd.autograd.linear_act is the differentiable form)."""
     dev = _half_inputs("linear_act", x, weight, bias, residual)
     a, x2, w2 = _linear_args("linear_act", x, weight, act)
@@ -1102,8 +1102,8 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
               b_up: Optional[torch.Tensor] = None, b_down: Optional[torch.Tensor] = None, act: str = "silu",
               residual: Optional[torch.Tensor] = None, keep: bool = False):
     """acmil_gated_ffn: y = (act(x @ w_gate^T + b_gate) * (x @ w_up^T + b_up)) @ w_down^T + b_down + residual, fp16 or bf16, in two products:
-    both projections with the activation and the gate, then the projection back with bias and residual (launches beside them as in linear_act).  x [..., D], w_gate and
-    w_up [F, D], w_down [D, F], residual [..., D]; act as linear_act ("silu" is the SwiGLU block, "gelu" GeGLU, "sigmoid" GLU, ...).
+    both projections with the activation and the gate, then the projection back with bias and residual (launches beside them as in linear_act).
+    x [..., D], w_gate and w_up [F, D], w_down [D, F], residual [..., D]; act as linear_act ("silu" is the SwiGLU block, "gelu" GeGLU, "sigmoid" GLU, ...).
     The gated features between the launches are held in x's type (in fp16, beyond 65504 they are infinite).  keep: also (g, u, h) for
     gated_ffn_bwd (g, u fp32 and h, each [rows, round8(F)]).  No gradient is recorded (acmil_amd.autograd.gated_ffn is the differentiable form)."""
     dev = _half_inputs("gated_ffn", x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual)
@@ -1134,7 +1134,8 @@ def gated_ffn_bwd(dy: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w_up:
                   need_down_bias: bool = False):
     """acmil_gated_ffn_bwd: (dx, dw_gate, dw_up, dw_down, db_gate, db_up, db_down) of gated_ffn for the incoming dy [..., D] and what
     gated_ffn(keep=True) kept; None where not asked for.  dw_gate / dw_up and db_gate / db_up are views of one buffer each.  The gradients of both
-    projections are held in the tensors' type between the products (in fp16, beyond 65504 infinite and below 2^-25 zero).  The residual's gradient is dy."""
+    projections are held in the tensors' type between the products (in fp16, beyond 65504 infinite and below 2^-25 zero).  The residual's gradient
+    is dy."""
     dev = _half_inputs("gated_ffn_bwd", x, w_gate, w_up, w_down, dy)
     a, hold = _ffn_args("gated_ffn_bwd", x, w_gate, w_up, w_down, act)
     if dy.shape != x.shape:

@@ -606,8 +606,8 @@ int acmil_adamw_step_peer(float* params, float* exp_avg, float* exp_avg_sq, long
  *     dz is held in the tensors' type for the products (db sums it before that rounding): in fp16, beyond 65504 it is infinite, and below 2^-25 it
  *     is lost.  The gradient of res is dy itself.
  *   acmil_gated_ffn       h = act(x Wg^T + bg) * (x Wu^T + bu);  y [M,D] = h Wd^T + bd + res    x [M,D], Wg, Wu [F,D], Wd [D,F]
- *     h is held in the tensors' type (the range of fp16 as above).  g, u (fp32 [M][round8(F)]) and h ([M][round8(F)] of dtype), 16-byte aligned: kept for the
- *     backward, all three or none (h then lives in the workspace).
+ *     h is held in the tensors' type (the range of fp16 as above).  g, u (fp32 [M][round8(F)]) and h ([M][round8(F)] of dtype), 16-byte
+ *     aligned: kept for the backward, all three or none (h then lives in the workspace).
  *   acmil_gated_ffn_bwd   dh = dy Wd, dg = dh u act'(g), du = dh act(g) (both held in the tensors' type, with its range);
  *     dx = dg Wg + du Wu; dWgu [2 round8(F)][D]: rows 0.. = dg^T x, rows round8(F).. = du^T x; dWd [D,F] = dy^T h;
  *     dbgu [2 round8(F)]: dbg, dbu likewise (sums of dg, du before they are rounded); dbd [D]  (each may be NULL; dense)
@@ -673,7 +673,8 @@ int acmil_gated_ffn_bwd(const acmil_ffn_args* args, void* workspace, size_t work
  * at most 2^-22 of itself and 2^-37 of |G|_F, which a step multiplies by up to a: less than an fp32 iteration keeps where a matrix holds
  * values of very different size.
  * A zero matrix gives zeros (eps > 0); infinities or NaN in g give NaN.  Reproducible bit for bit for the same list of matrices (a matrix beside
- * others may be multiplied in other tiles, and differ in its last bits from one alone).  But for o = g, no output may overlap another matrix of the call.
+ * others may be multiplied in other tiles, and differ in its last bits from one alone).  But for o = g, no output may
+ * overlap a matrix of the call.
  * workspace: acmil_orthogonalize_workspace_bytes(...) (0 = refused), 256-byte aligned, contents arbitrary.
  * ------------------------------------------------------------------------------------------- */
 typedef struct acmil_ortho_mat {
